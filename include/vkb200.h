@@ -450,6 +450,173 @@ VKB_API vkb_status vkb_session_copy_stream(vkb_session* s, int32_t src, int32_t 
 VKB_API vkb_status vkb_log_mel(vkb_context* ctx, const float* pcm_dev, int64_t n_clips, int64_t stride,
                                const int32_t* lengths_dev, int32_t n_mels, float* out_dev);
 
+/* ---- rules on logits and the choice of tokens ------------------------------
+ * What stands between a decoder's logits and its next token. For row r and
+ * token j that occurs c times in the row's history:
+ *   x = logits[r][j]
+ *   c > 0:  x = (x > 0 ? x / repetition[r] : x * repetition[r])
+ *               - (frequency[r] * c + presence[r])
+ *   x = x + bias[bias_row[r]][j]
+ *   x = -inf where j would complete an n-gram that the history already has, or
+ *       where bit j of mask[mask_row[r]] is clear (bit j % 32 of word j / 32)
+ * each operation one fp32 rounding, in this order. Every pointer may be NULL:
+ * no history, repetition 1, frequency and presence 0, no bias, no mask. The
+ * reference has the n-gram rule on the host (crates/vokra-core/src/decode/
+ * beam_search.rs:442-476) and none of the others. */
+typedef struct vkb_logits_rules {
+    const int32_t* hist_dev;       /* [rows][hist_ld] token ids; ids outside the vocabulary count for nothing */
+    int64_t hist_ld;
+    const int32_t* hist_len_dev;   /* [rows] valid ids of each row (clipped to hist_ld); NULL = hist_ld */
+    const float* repetition_dev;   /* [rows] */
+    const float* frequency_dev;    /* [rows] */
+    const float* presence_dev;     /* [rows] */
+    int32_t no_repeat_ngram;       /* n of the n-gram rule; 0 or 1 = off */
+    int32_t n_bias;                /* rows of the bias table */
+    const float* bias_dev;         /* [n_bias][bias_ld] */
+    int64_t bias_ld;
+    const int32_t* bias_row_dev;   /* [rows]; outside 0..n_bias-1 = no bias; NULL = row 0 for every row */
+    const uint32_t* mask_dev;      /* [n_mask][mask_ld] words (one row for each grammar state, say) */
+    int64_t mask_ld;
+    const int32_t* mask_row_dev;   /* [rows]; outside 0..n_mask-1 = no mask; NULL = row 0 for every row */
+    int32_t n_mask;
+} vkb_logits_rules;
+
+/* out[r][j] = the logits after the rules (NULL rules: a copy), rounded once to
+ * `dtype` (VKB_DT_F32 or VKB_DT_F16, the type of both). out_dev may be
+ * logits_dev itself (then out_ld == ld); other overlaps are not allowed.
+ * ld and out_ld are in elements. */
+VKB_API vkb_status vkb_logits_process(vkb_context* ctx, const void* logits_dev, int32_t dtype, int64_t n_rows,
+                                      int64_t n_vocab, int64_t ld, const vkb_logits_rules* rules, void* out_dev,
+                                      int64_t out_ld);
+
+/* The k best tokens of each row after the rules, without writing the logits:
+ * ids [n_rows][k] and log-probabilities [n_rows][k] (log-softmax over the
+ * row), the best first, equal values by the lower id. A token at -inf is never
+ * chosen, nor one whose value is not a number (both count nothing in the
+ * softmax): where fewer than k are left the rest is id -1, log-probability
+ * -inf. A row with +inf shares its probability among the tokens at +inf.
+ * k = 1 is the greedy choice. The result does not depend on how the row is
+ * split over the GPU beyond the last bits of the log-probability. */
+#define VKB_LOGITS_TOPK_MAX 64
+VKB_API vkb_status vkb_logits_topk(vkb_context* ctx, const void* logits_dev, int32_t dtype, int64_t n_rows,
+                                   int64_t n_vocab, int64_t ld, const vkb_logits_rules* rules, int32_t k,
+                                   int32_t* ids_dev, float* logprob_dev);
+
+/* ---- paged KV cache in 8 bits, one scale per block of 16 tokens and head ---
+ * Storage and page tables belong to the caller and lie on the device, so that
+ * a step (fork, grow, append, attend) needs no word from the host. One page
+ * holds 16 tokens of one stream for every head:
+ *   k [n_layer][n_pages][n_kv_head][16][d_head]   int8
+ *   v [n_layer][n_pages][n_kv_head][d_head][16]   int8 (a channel's tokens together)
+ *   k_scale, v_scale [n_layer][n_pages][n_kv_head]  f32; value = quant * scale
+ * d_head is 32, 64, 96, 128 or 256. Half the bytes of an f16 cache; against
+ * VKB_KV_Q8_0 pages it has 8 bytes of scales per 16 tokens and head where those
+ * have 64 (d_head 64), and grouped heads. */
+#define VKB_BKV_BLOCK 16
+#define VKB_BKV_MAX_SEQ 8192
+typedef struct vkb_bkv_cache {
+    int32_t n_layer, n_kv_head, d_head;
+    int64_t n_pages;
+    void* k_dev;
+    void* v_dev;
+    float* k_scale_dev;
+    float* v_scale_dev;
+} vkb_bkv_cache;
+
+/* The streams of one call. Stream s owns rows tok_start[s] .. tok_start[s+1]-1
+ * of the call's row arrays; they are its last rows: the last one is at
+ * position kv_len[s] - 1. Page p of the stream is table[s * table_ld + p]; an id
+ * outside 0..n_pages-1 is a page that is not there: it is never written, and
+ * its tokens are not seen. n_tok = tok_start[n_seq]; max_q is the largest
+ * number of rows of one stream (a hint for the launch: a wrong one costs time). */
+typedef struct vkb_bkv_batch {
+    int32_t n_seq, n_tok, max_q;
+    const int32_t* tok_start_dev;  /* [n_seq + 1] */
+    const int32_t* kv_len_dev;     /* [n_seq] tokens of the stream, this call's included */
+    const int32_t* table_dev;      /* [n_seq][table_ld] */
+    int64_t table_ld;
+    const int32_t* status_dev;     /* NULL, or vkb_pages_advance's status: where it is not 0, nothing is appended */
+} vkb_bkv_batch;
+
+/* Stores the batch's rows of K and V ([n_tok] rows of n_kv_head*d_head values,
+ * row strides in elements, VKB_DT_F32 or VKB_DT_F16). Block by block: s' =
+ * max(s, amax/127), where s is the block's scale, or 0 when its first slot is
+ * among the new rows; earlier quants become rint(q * (s/s')), new ones
+ * rint(x * (1/s')), in IEEE fp32. NaN is stored as 0, an infinity as the
+ * largest value of a block whose scale is FLT_MAX/127. A page must not be
+ * shared with another stream (vkb_pages_advance copies shared ones first). */
+VKB_API vkb_status vkb_bkv_append(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,
+                                  const vkb_bkv_batch* batch, const void* k_dev, int64_t k_ld, const void* v_dev,
+                                  int64_t v_ld, int32_t dtype);
+
+/* Causal attention of the batch's rows over their streams' caches:
+ * out = softmax(scale * q . K) V per head, over the keys at positions up to the
+ * row's own. Query head j reads KV head j / (n_head / n_kv_head). q and out:
+ * [n_tok] rows of n_head*d_head values, row strides in elements, F32 or F16
+ * each. With an F32 q or out the products are accurate to about 2^-21, else
+ * q and the weights enter them as f16; sums and statistics are fp32 either
+ * way. A row without keys (a stream of length 0) is zero. */
+VKB_API vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,
+                                     const vkb_bkv_batch* batch, int32_t n_head, const void* q_dev, int64_t q_ld,
+                                     int32_t q_dtype, float scale, void* out_dev, int64_t out_ld, int32_t out_dtype);
+
+/* The stored values of each stream's last rows (the batch's rows), K and V,
+ * [n_tok][n_kv_head][d_head] in `dtype`; rows before position 0 and tokens of
+ * pages that are not there are zero. */
+VKB_API vkb_status vkb_bkv_read(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,
+                                const vkb_bkv_batch* batch, void* k_dev, void* v_dev, int32_t dtype);
+
+/* ---- the pages of such a cache: fork, free, grow, compact ------------------
+ * Works on any paged storage: a plane is one array of pages for each layer. The
+ * page tables, lengths and reference counts (how many tables list a page) are
+ * a state; a call reads one and writes another one, whose arrays must not
+ * overlap the first's, so a step can be repeated or given up. */
+#define VKB_PAGES_MAX_PLANES 8
+typedef struct vkb_page_plane {
+    void* base_dev;      /* page i of layer l is at base + l*layer_bytes + i*page_bytes */
+    int64_t page_bytes;
+    int64_t layer_bytes;
+} vkb_page_plane;
+typedef struct vkb_page_pool {
+    int32_t n_layer, n_planes;
+    const vkb_page_plane* planes;  /* host array */
+    int64_t n_pages;
+    int32_t n_seq, page_tokens;
+    int64_t table_ld;
+    int32_t* status_dev;           /* one int32: vkb_pages_advance raises it, the caller clears it */
+} vkb_page_pool;
+typedef struct vkb_page_state {
+    int32_t* table_dev;  /* [n_seq][table_ld], -1 behind a stream's last page */
+    int32_t* len_dev;    /* [n_seq] tokens */
+    int32_t* refs_dev;   /* [n_pages] */
+} vkb_page_state;
+enum vkb_page_status {
+    VKB_PAGES_OK = 0,
+    VKB_PAGES_EXHAUSTED = 1,  /* too few free pages */
+    VKB_PAGES_TABLE_FULL = 2, /* a stream would be longer than table_ld pages */
+    VKB_PAGES_BAD_INPUT = 3   /* a parent >= n_seq, a negative n_new or length, a table entry outside the arena */
+};
+
+/* One step of every stream, decided and done on the device:
+ *   stream i becomes stream parent[i] of `from` (its pages are shared, not
+ *   copied; parent < 0 frees the stream; NULL = every stream stays), then
+ *   grows by n_new[i] tokens (NULL = 0; freed streams do not grow): pages are
+ *   added, and a partly filled last page that other streams share is copied
+ *   to a page of the stream's own, every layer of it, before it is written.
+ * New pages are the lowest ones that are free both in `from` and after the
+ * fork, taken by the streams in order (a copy first); so `from` stays valid,
+ * and pages that this call frees serve the next one. If the call cannot be
+ * done, *status_dev says why (vkb_page_status), no page is touched and `to` is
+ * a copy of `from`. */
+VKB_API vkb_status vkb_pages_advance(vkb_context* ctx, const vkb_page_pool* pool, const int32_t* parent_dev,
+                                     const int32_t* n_new_dev, const vkb_page_state* from, const vkb_page_state* to);
+
+/* Moves pages so that the n pages in use are pages 0 .. n-1: the i-th page in
+ * use at or behind n goes to the i-th free page before n. Writes the new
+ * tables, lengths and counts to `to` and n to n_used_dev (may be NULL). */
+VKB_API vkb_status vkb_pages_compact(vkb_context* ctx, const vkb_page_pool* pool, const vkb_page_state* from,
+                                     const vkb_page_state* to, int32_t* n_used_dev);
+
 #ifdef __cplusplus
 }
 #endif

@@ -78,6 +78,46 @@ class WhisperDims(C.Structure):
     ]
 
 
+class LogitsRules(C.Structure):
+    _fields_ = [
+        ("hist", C.c_void_p), ("hist_ld", C.c_int64), ("hist_len", C.c_void_p), ("repetition", C.c_void_p),
+        ("frequency", C.c_void_p), ("presence", C.c_void_p), ("no_repeat_ngram", C.c_int32), ("n_bias", C.c_int32),
+        ("bias", C.c_void_p), ("bias_ld", C.c_int64), ("bias_row", C.c_void_p), ("mask", C.c_void_p),
+        ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("n_mask", C.c_int32),
+    ]
+
+
+LOGITS_TOPK_MAX = 64
+BKV_BLOCK = 16
+BKV_MAX_SEQ = 8192
+
+
+class BkvCache(C.Structure):
+    _fields_ = [("n_layer", C.c_int32), ("n_kv_head", C.c_int32), ("d_head", C.c_int32), ("n_pages", C.c_int64),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+class BkvBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_int32), ("n_tok", C.c_int32), ("max_q", C.c_int32), ("tok_start", C.c_void_p),
+                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int64), ("status", C.c_void_p)]
+
+
+class PagePlane(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("page_bytes", C.c_int64), ("layer_bytes", C.c_int64)]
+
+
+class PagePool(C.Structure):
+    _fields_ = [("n_layer", C.c_int32), ("n_planes", C.c_int32), ("planes", C.POINTER(PagePlane)),
+                ("n_pages", C.c_int64), ("n_seq", C.c_int32), ("page_tokens", C.c_int32), ("table_ld", C.c_int64),
+                ("status", C.c_void_p)]
+
+
+class PageState(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("len", C.c_void_p), ("refs", C.c_void_p)]
+
+
+PAGES_OK, PAGES_EXHAUSTED, PAGES_TABLE_FULL, PAGES_BAD_INPUT = 0, 1, 2, 3
+
 P = C.c_void_p
 I32, I64, U32, U64, SZ, F32 = C.c_int32, C.c_int64, C.c_uint32, C.c_uint64, C.c_size_t, C.c_float
 PP = C.POINTER(C.c_void_p)
@@ -140,6 +180,13 @@ SIGNATURES = {
     "vkb_session_logits": (P, [P]),
     "vkb_session_ids": (P, [P]),
     "vkb_session_release": (C.c_int, [P, I32]),
+    "vkb_logits_process": (C.c_int, [P, P, I32, I64, I64, I64, P, P, I64]),
+    "vkb_logits_topk": (C.c_int, [P, P, I32, I64, I64, I64, P, I32, P, P]),
+    "vkb_bkv_append": (C.c_int, [P, P, I32, P, P, I64, P, I64, I32]),
+    "vkb_bkv_attention": (C.c_int, [P, P, I32, P, I32, P, I64, I32, F32, P, I64, I32]),
+    "vkb_bkv_read": (C.c_int, [P, P, I32, P, P, P, I32]),
+    "vkb_pages_advance": (C.c_int, [P, P, P, P, P, P]),
+    "vkb_pages_compact": (C.c_int, [P, P, P, P, P]),
 }
 
 _lib = None
