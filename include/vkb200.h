@@ -540,9 +540,9 @@ typedef struct vkb_bkv_batch {
 
 /* Stores the batch's rows of K and V ([n_tok] rows of n_kv_head*d_head values,
  * row strides in elements, VKB_DT_F32 or VKB_DT_F16). Block by block: s' =
- * max(s, amax/127), where s is the block's scale, or 0 when its first slot is
- * among the new rows; earlier quants become rint(q * (s/s')), new ones
- * rint(x * (1/s')), in IEEE fp32. NaN is stored as 0, an infinity as the
+ * max(s, amax * (1/127)), where s is the block's scale, or 0 when its first
+ * slot is among the new rows; earlier quants become rint(q * (s/s')), new ones
+ * rint(x * (1/s')), each operation in IEEE fp32 (1/127 too is one fp32 number). NaN is stored as 0, an infinity as the
  * largest value of a block whose scale is FLT_MAX/127. A page must not be
  * shared with another stream (vkb_pages_advance copies shared ones first). */
 VKB_API vkb_status vkb_bkv_append(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,

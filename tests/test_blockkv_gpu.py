@@ -45,7 +45,7 @@ class Plain:
                         amax = np.minimum(np.fmax.reduce(np.fmax.reduce(np.abs(x), 2), 1), np.finfo(np.float32).max)
                         amax = np.fmax(amax, one(0))
                         old = sc.copy() if t0 > 0 else np.zeros_like(sc)
-                        new = np.maximum(old, amax / one(127))
+                        new = np.maximum(old, amax * (one(1) / one(127)))
                         inv = np.where(new > 0, one(1) / new, one(0)).astype(np.float32)
                         grown = (new > old)[:, None, None] & (t0 > 0)
                         ratio = np.where(new > 0, old / new, one(0)).astype(np.float32)

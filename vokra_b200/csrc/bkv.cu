@@ -5,7 +5,7 @@
 // [d_head][16] (a channel's tokens together), which is how the attention's
 // matrix instructions take the two, so neither is ever transposed on the way.
 //
-// append, block by block: s' = max(s, amax / 127) with s = 0 where the block's
+// append, block by block: s' = max(s, amax * (1/127)) with s = 0 where the block's
 // first slot is among the new tokens; the block's earlier quants become
 // rint(q * (s / s')) where s' > s, the new ones rint(x * (1 / s')). All in
 // IEEE fp32, so the stored bytes are defined to the bit. NaN counts as 0 and
@@ -141,6 +141,7 @@ __device__ __forceinline__ int8_t quant(float x, float inv) {
 }
 
 constexpr int APPEND_WARPS = 4;
+constexpr float SCALE = 1.0f / 127.0f;  // rounded to fp32: part of the definition
 
 // grid (2 * n_kv_head / 4, pages of a stream, streams); warp = one head and side.
 template <typename T, int D, bool VEC>
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS)
                 for (int c = 0; c < C; ++c) amax = fmaxf(amax, fabsf(x[t][c]));
             }
         amax = fminf(warp_max(amax), FLT_MAX);
-        const float s_new = fmaxf(s_old, __fdiv_rn(amax, 127.0f));
+        const float s_new = fmaxf(s_old, amax * SCALE);
         const float inv = s_new > 0.0f ? __fdiv_rn(1.0f, s_new) : 0.0f;
         const bool grown = t0 > 0 && s_new > s_old;
         const float ratio = grown ? __fdiv_rn(s_old, s_new) : 1.0f;
