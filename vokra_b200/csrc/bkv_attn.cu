@@ -2,40 +2,44 @@
 // rows a stream: decode steps, tokens to check, short chunks.
 //
 // Bound: HBM (2 d_head bytes a key and KV head). A warp takes 64 keys = 4 pages
-// at a time and feeds m16n8k16 tensor-core products straight from global
-// memory: no shared memory, no transpose, and every 16-byte load is used whole.
-// What makes that work is that the order of keys and channels inside a product
-// is free as long as both operands agree:
-//  - lane (g, c) = (lane / 4, lane % 4). Column n of the score tile t is token
+// at a time from a ring of its own in shared memory, filled by bulk copies that
+// run ahead over the ends of its items; pages are contiguous, and neither K nor
+// V is ever transposed or shuffled. What makes that work is that the order of
+// keys and channels inside a matrix product is free as long as both operands
+// agree:
+//  - lane (g, c) = (lane / 4, lane % 4). Column n of score tile t is token
 //    2t + n % 2 of page n / 2, so that lane c's columns (2c, 2c + 1) of all 8
-//    tiles are the 16 tokens of page c: one K scale, one V scale and one page
-//    id a lane and step.
-//  - a K row is loaded as 16 neighbouring channels a lane (D = 64: a quad reads
-//    the 64 bytes of a key, a warp 4 x 128 bytes), which are four k steps of the
-//    Q.K product; q is kept in the same order.
-//  - V is stored channel by channel, so 16 bytes at (page c, channel 8i + g) are
-//    the 16 tokens whose weights the lane holds: four k steps of the P.V product.
-// int8 -> f16 is exact (a byte permute into 1024 + u, minus 1152). The K scale
-// multiplies the scores, the V scale the weights, both in fp32; weights enter
-// the product divided by a running power of two above the V scales, so that f16
-// holds them whatever the scale.
+//    tiles are the 16 tokens of page c: one K scale and one V scale a lane.
+//  - a lane reads 16 neighbouring channels of a K row: two k steps (m16n8k32,
+//    int8) of Q.K. q is made int8 planes in the same order: p1 + p2 / 254 (+
+//    p3 / 254^2) units of 1/127 of the row's largest. The products are exact
+//    in 32-bit integers; two planes hold q to 2^-16 of that largest, three to
+//    2^-24. K is never converted, which was a third of the instructions.
+//  - V is stored channel by channel, so 16 bytes of (page c, channel 8i + g) are
+//    the 16 tokens whose weights the lane holds: four k steps of P.V (m16n8k16).
+//    int8 -> f16 is exact (a byte permute into 1024 + u, minus 1152). The V scale
+//    multiplies the weights in fp32; weights enter divided by a running power of
+//    two above the V scales, so that f16 holds them whatever the scale.
 //
-// SPLIT tiles (8 query rows) hold the high f16 part of q in rows 0..7 of the
-// 16-row operand and the low part in rows 8..15, likewise for the weights: the
-// products are accurate to about 2^-21 at the price of one. Tiles of 16 rows
-// have one f16 part. Up to 8 rows SPLIT costs nothing more and is taken always.
+// Tiles of 8 query rows (SPLIT) hold p1 in rows 0..7 of the 16-row operand and
+// p2 in rows 8..15, likewise the high and low f16 parts of the weights: 2^-21
+// at the price of one product. 32-bit rows take the third plane in a second
+// one. Tiles of 16 rows (16-bit rows, more than 8 a stream and KV head) take
+// two products for the planes and one f16 part of the weights.
 //
 // The (stream, KV head, row tile, 64 keys) steps of the whole call are one
-// sequence, cut into equal contiguous ranges, one a warp, so ragged lengths
-// balance themselves. A warp finishes an item that lies in its range alone;
-// the others leave partial rows that bkv_combine_kernel joins in order.
+// sequence, cut into equal contiguous shares for the blocks and their warps, so
+// ragged lengths balance themselves. A warp finishes an item that lies in its
+// share alone; parts of shared items are joined in order, first within the
+// block, then by the last block of the item to arrive.
 #include "bkv.cuh"
+#include "tc_ptx.cuh"
 #include <algorithm>
 
 namespace vkb {
 namespace {
 
-constexpr int AW = 4;  // warps of a block
+constexpr int BKV_SEQ_PER_LAUNCH = 512;
 constexpr float L2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -46,9 +50,29 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Four values y (in units of 1/127 of the row's largest) as int8 words: the nearest whole numbers, then 254 times
+// what they leave, and so on; y becomes what is left behind the word, times 254.
+__device__ __forceinline__ uint32_t take_plane(float (&y)[4]) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int q = __float2int_rn(y[e]);
+        w |= (uint32_t)(q & 0xff) << (8 * e);
+        y[e] = (y[e] - (float)q) * 254.0f;
+    }
+    return w;
 }
 
 // Four int8 (one word) as two f16 pairs: bytes 0, 1 and bytes 2, 3.
@@ -80,449 +104,717 @@ struct AttnArgs {
     float scale;
     void* out;
     int64_t out_ld;
-    int q_f16, out_f16, q_vec;
-    float* part_o;   // [warps][2][rows][D]
-    float2* part_ml; // [warps][2][rows]
-    int4* todo;      // [warps]: the item that starts in the warp's range and goes on behind it (stream, head,
-                     // tile, further warps * 2 + slot of its first part); stream -1: none
+    int q_f16, out_f16, q_vec, out_vec;
+    float* warp_o;    // [blocks * AW][2][rows][D]: a warp's parts of items that it shares with others
+    float2* warp_ml;  // [blocks * AW][2][rows]
+    float* block_o;   // [blocks][2][rows][D]: the same of a block
+    float2* block_ml;
+    unsigned* arrived;  // [blocks], 0 at rest: blocks that have left their part of the item that starts in block i
+    int* err;
 };
 
-__device__ __forceinline__ int64_t steps_of(const AttnArgs& A, int s, int tile_rows, int& tiles, int& chunks) {
-    int first, n;
-    A.S.rows(s, first, n);
-    tiles = (n * A.group + tile_rows - 1) / tile_rows;
-    chunks = max(1, (A.S.keys(s) + 63) / 64);
-    return (int64_t)A.L.n_kv_head * tiles * chunks;
-}
+// What a block knows of the streams: the running number of steps in front of
+// each (pre[n_seq] is the total), keys, first row.
+struct Streams {
+    int64_t pre[BKV_SEQ_PER_LAUNCH + 1];
+    int keys[BKV_SEQ_PER_LAUNCH];
+    int first[BKV_SEQ_PER_LAUNCH];
+    int n_q[BKV_SEQ_PER_LAUNCH];
+};
 
-// Running steps in front of each stream, in shared memory: pre[n_seq] is the total.
-template <int TR>
-__device__ __forceinline__ void stream_prefix(const AttnArgs& A, int64_t* pre) {
-    __shared__ int64_t warp_sum_s[32];
-    __shared__ int64_t carry_s;
+template <int D>
+struct Ring {
+    // Warps of a block, one block an SM, and the ring's slots of each. 64 streams of up to 448 keys, 20 heads of 64:
+    // 12 warps x 4 slots 29.3 us, 16 x 3 34.8 (spills), 8 x 5 33.2; one stream of 131071 keys, 8 heads of 128: 8 x 3
+    // 73 us, 10 x 2 93, 12 x 2 81 (before the int8 scores).
+    static constexpr int AW = D <= 64 ? 12 : D <= 128 ? 8 : 4;
+    static constexpr int PAGE = BKV_BLOCK * D;
+    static constexpr int STRIDE = PAGE + 32;    // pages of a slot: the 32 bytes spread a quad's V loads over the banks
+    static constexpr int SLOT = 4 * STRIDE;     // the K or the V of 64 keys
+    static constexpr int SLOTS = D <= 64 ? 4 : 3;
+    static constexpr int META = 8;
+    static constexpr int WARP = SLOTS * SLOT + META * 4 * (int)sizeof(int) + SLOTS * (int)sizeof(uint64_t) + 8;
+    static constexpr int WARP_BYTES = (WARP + 15) / 16 * 16;
+};
+
+template <int TR, int AW>
+__device__ __forceinline__ void load_streams(const AttnArgs& A, Streams& st) {
+    __shared__ int64_t sums[AW];
     const int n = A.S.n_seq, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) {
-        carry_s = 0;
-        pre[0] = 0;
-    }
-    __syncthreads();
-    for (int base = 0; base < n; base += blockDim.x) {
+    int64_t carry = 0;
+    if (threadIdx.x == 0) st.pre[0] = 0;
+    for (int base = 0; base < n; base += 32 * AW) {
         const int s = base + (int)threadIdx.x;
-        int tiles, chunks;
-        int64_t x = s < n ? steps_of(A, s, TR, tiles, chunks) : 0;
+        int64_t x = 0;
+        if (s < n) {
+            int first, rows;
+            A.S.rows(s, first, rows);
+            const int keys = A.S.keys(s);
+            st.keys[s] = keys;
+            st.first[s] = first;
+            st.n_q[s] = rows;
+            x = (int64_t)A.L.n_kv_head * ((rows * A.group + TR - 1) / TR) * max(1, (keys + 63) / 64);
+        }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        if (lane == 31) warp_sum_s[warp] = x;
+        if (lane == 31) sums[warp] = x;
         __syncthreads();
-        int64_t before = carry_s;
-        for (int w = 0; w < warp; ++w) before += warp_sum_s[w];
-        if (s < n) pre[s + 1] = before + x;
-        __syncthreads();
-        if ((int)threadIdx.x == blockDim.x - 1) carry_s = before + x;
+        int64_t all = 0;
+#pragma unroll
+        for (int w = 0; w < AW; ++w) {
+            if (w < warp) x += sums[w];
+            all += sums[w];
+        }
+        if (s < n) st.pre[s + 1] = carry + x;
+        carry += all;
         __syncthreads();
     }
 }
 
-template <int D, bool SPLIT>
-__global__ void __launch_bounds__(32 * AW, D <= 64 ? 3 : D <= 128 ? 2 : 1) bkv_attn_kernel(AttnArgs A) {
+// A place in the sequence of steps (stream, KV head, row tile, 64 keys).
+template <int TR>
+struct Walk {
+    int64_t u;      // the step
+    int s, h, tile, ch;
+    int tiles, chunks;
+    int seen;       // steps of the item in which some row sees a key
+
+    __device__ __forceinline__ void stream(const AttnArgs& A, const Streams& st) {
+        tiles = (st.n_q[s] * A.group + TR - 1) / TR;
+        chunks = max(1, (st.keys[s] + 63) / 64);
+    }
+    __device__ __forceinline__ void item(const AttnArgs& A, const Streams& st) {
+        const int last_tok = min(st.n_q[s] * A.group, (tile + 1) * TR) - 1;
+        const int keys = max(0, st.keys[s] - st.n_q[s] + last_tok / A.group + 1);
+        seen = (keys + 63) / 64;
+    }
+    __device__ __forceinline__ void seek(const AttnArgs& A, const Streams& st, int64_t to) {
+        u = to;
+        int lo = 0, hi = A.S.n_seq - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (st.pre[mid] <= to) lo = mid;
+            else hi = mid - 1;
+        }
+        s = lo;
+        while (st.pre[s + 1] <= to) ++s;
+        stream(A, st);
+        const int64_t in_seq = to - st.pre[s];
+        const int64_t i = in_seq >> 32 ? in_seq / chunks : (uint32_t)in_seq / (uint32_t)chunks;
+        ch = (int)(in_seq - i * chunks);
+        h = (int)(i >> 32 ? i / tiles : (uint32_t)i / (uint32_t)tiles);
+        tile = (int)(i - (int64_t)h * tiles);
+        item(A, st);
+    }
+    // On to the item's next step, or (past its end) to the next item, if there is one before `end`.
+    __device__ __forceinline__ void next_item(const AttnArgs& A, const Streams& st, int64_t end) {
+        ch = 0;
+        if (++tile == tiles) {
+            tile = 0;
+            if (++h == A.L.n_kv_head) {
+                h = 0;
+                if (u < end) {
+                    ++s;
+                    while (st.pre[s + 1] <= u) ++s;
+                    stream(A, st);
+                }
+            }
+        }
+        item(A, st);
+    }
+    // The next step that has keys to load; false: none before `end`.
+    __device__ __forceinline__ bool to_loaded(const AttnArgs& A, const Streams& st, int64_t end) {
+        while (u < end && ch >= seen) {
+            u += chunks - ch;
+            next_item(A, st, end);
+        }
+        return u < end;
+    }
+    __device__ __forceinline__ void step(const AttnArgs& A, const Streams& st, int64_t end) {
+        ++u;
+        if (++ch == chunks) next_item(A, st, end);
+    }
+};
+
+// A part of an item that several warps share.
+struct Part {
+    int64_t u0;  // the item's first step
+    int chunks;  // its steps; 0: no part
+    int s, h, tile;
+    int head;    // the first one of its item in the block
+};
+
+__device__ __forceinline__ void store_pair(const AttnArgs& A, int64_t at, float y0, float y1) {
+    if (A.out_f16) {
+        __half* p = reinterpret_cast<__half*>(A.out) + at;
+        if (A.out_vec) {
+            *reinterpret_cast<__half2*>(p) = __floats2half2_rn(y0, y1);
+        } else {
+            p[0] = __float2half_rn(y0);
+            p[1] = __float2half_rn(y1);
+        }
+    } else {
+        float* p = reinterpret_cast<float*>(A.out) + at;
+        if (A.out_vec) {
+            *reinterpret_cast<float2*>(p) = make_float2(y0, y1);
+        } else {
+            p[0] = y0;
+            p[1] = y1;
+        }
+    }
+}
+
+// Joins row r of `n` parts, in order, a warp a row; part i's rows are o(i) and their (max, sum) ml(i). To the
+// output, or (to_o) to another part.
+template <int D, class FO, class FM>
+__device__ __forceinline__ void join_row(const AttnArgs& A, int n, int r, int64_t row_at, int tile_row0, int h, FO o, FM ml,
+                                         float* to_o, float2* to_ml) {
+    const int lane = threadIdx.x & 31;
+    constexpr int C = D / 32;  // channels of a lane, as pairs 64 apart (one alone for D = 32, three for D = 96)
+    float m = -INFINITY, l = 0.0f, y[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) y[i] = 0.0f;
+    auto ch = [&](int i) { return C == 1 ? lane : C % 2 ? lane + 32 * i : 64 * (i / 2) + 2 * lane + i % 2; };
+    constexpr int U = C <= 4 ? 8 : 4;
+    for (int p0 = 0; p0 < n; p0 += U) {
+        float2 x[U];
+        float v[U][C];
+#pragma unroll
+        for (int p = 0; p < U; ++p) {
+            const bool real = p0 + p < n;
+            x[p] = real ? __ldcg(ml(p0 + p) + r) : make_float2(-INFINITY, 0.0f);
+            const float* row = o(real ? p0 + p : 0) + r * D;
+#pragma unroll
+            for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
+                if constexpr (C % 2) {
+                    v[p][i] = __ldcg(row + ch(i));
+                } else {
+                    const float2 f = __ldcg(reinterpret_cast<const float2*>(row + ch(i)));
+                    v[p][i] = f.x;
+                    v[p][i + 1] = f.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < U; ++p) {
+            const float m_new = fmaxf(m, x[p].x);
+            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+            const float a = ex2(m - m_use), b = ex2(x[p].x - m_use);
+            l = l * a + x[p].y * b;
+#pragma unroll
+            for (int i = 0; i < C; ++i) y[i] = y[i] * a + (p0 + p < n ? v[p][i] : 0.0f) * b;
+            m = m_new;
+        }
+    }
+    if (to_o) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) to_o[r * D + ch(i)] = y[i];
+        if (lane == 0) to_ml[r] = make_float2(m, l);
+    } else {
+        const int row = tile_row0 + r, tok = row / A.group, head = h * A.group + row % A.group;
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const int64_t at = (row_at + tok) * A.out_ld + (int64_t)head * D;
+#pragma unroll
+        for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
+            if constexpr (C % 2) {
+                if (A.out_f16) reinterpret_cast<__half*>(A.out)[at + ch(i)] = __float2half_rn(y[i] * inv);
+                else reinterpret_cast<float*>(A.out)[at + ch(i)] = y[i] * inv;
+            } else {
+                store_pair(A, at + ch(i), y[i] * inv, y[i + 1] * inv);
+            }
+        }
+    }
+}
+
+template <int D, bool SPLIT, bool P3>
+__global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs A) {
     pdl_entry();
     constexpr int TR = SPLIT ? 8 : 16;       // query rows of a tile
     constexpr int NR = SPLIT ? 1 : 2;        // of them in this lane's hands
     constexpr int KW = D / 16;               // 32-bit words of a K row a lane holds = k steps of Q.K
     constexpr int NT = D / 8;                // channel tiles of P.V
-    extern __shared__ int64_t pre[];         // [n_seq + 1]
-    stream_prefix<TR>(A, pre);
-    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-    const int64_t n_warps = (int64_t)gridDim.x * AW;
-    const int64_t me = (int64_t)blockIdx.x * AW + (threadIdx.x >> 5);
-    const int64_t total = pre[A.S.n_seq];
-    const int64_t per = (total + n_warps - 1) / n_warps;
-    const int64_t u_begin = min(total, me * per), u_end = min(total, u_begin + per);
-    if (lane == 0) A.todo[me] = make_int4(-1, 0, 0, 0);
-    if (u_begin == u_end) return;
-
-    // the stream of the first step
-    int s;
-    {
-        int lo = 0, hi = A.S.n_seq - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (pre[mid] <= u_begin) lo = mid;
-            else hi = mid - 1;
-        }
-        s = lo;
+    using R = Ring<D>;
+    constexpr int AW = R::AW;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Streams& st = *reinterpret_cast<Streams*>(smem);
+    __shared__ Part parts[2 * AW];
+    __shared__ int last_one[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    uint8_t* mine = smem + (sizeof(Streams) + 15) / 16 * 16 + (size_t)warp * R::WARP_BYTES;
+    int* meta = reinterpret_cast<int*>(mine + R::SLOTS * R::SLOT);  // [META][4] ids of a step's pages
+    uint64_t* full = reinterpret_cast<uint64_t*>(meta + R::META * 4);
+    if (lane == 0) {
+        for (int i = 0; i < R::SLOTS; ++i) ptx::mbar_init(&full[i], 1);
+        ptx::fence_mbar_init();
     }
-    int64_t u = u_begin;
-    while (u < u_end) {
-        while (pre[s + 1] <= u) ++s;
-        int tiles, chunks;
-        steps_of(A, s, TR, tiles, chunks);
-        int first_row, n_q;
-        A.S.rows(s, first_row, n_q);
-        const int64_t in_seq = u - pre[s];
-        const int item = (int)(in_seq / chunks);
-        const int c0 = (int)(in_seq % chunks);
-        const int c1 = (int)min((int64_t)chunks, c0 + (u_end - u));
-        const int h = item / tiles, tile = item % tiles;
-        const int n_keys = A.S.keys(s);
+    if (lane < 2) parts[2 * warp + lane].chunks = 0;
+    load_streams<TR, AW>(A, st);
+    __syncthreads();
+    const int64_t total = st.pre[A.S.n_seq];
+    // equal shares for the blocks (fewer of them where the warps would not get a step each) and their warps
+    const int64_t n_block = min((int64_t)gridDim.x, (total + AW - 1) / AW);
+    if (blockIdx.x >= n_block) return;
+    const int64_t block_begin = blockIdx.x * total / n_block, block_end = (blockIdx.x + 1) * total / n_block;
+    // warps without a step are the block's last ones: an item's warps follow one another
+    const int64_t share = (block_end - block_begin) / AW;
+    const int rest = (int)((block_end - block_begin) % AW);
+    const int64_t u_begin = block_begin + warp * share + min(warp, rest), u_end = u_begin + share + (warp < rest ? 1 : 0);
+    bool ok = true;
 
-        // ---- the tile's query rows: f16 operands in the order of the K loads
-        uint32_t qa[KW][4];
-        float row_fac[NR];  // multiplies a score: 2^e * scale * log2(e)
-        int limit[NR];      // keys that the row sees
+    if (u_begin < u_end) {
+        // ---- the loads run ahead of the products by R::SLOTS halves of a step, over the ends of items
+        Walk<TR> ld;
+        ld.seek(A, st, u_begin);
+        Walk<TR> w = ld;
+        bool more = ld.to_loaded(A, st, u_end);
+        int ids = -1, ids_s = -1, ids_b = 0;  // lane i: page 32 * ids_b + i of stream ids_s
+        int page = -1;
+        int op = 0;  // the next half step to load: even K, odd V
+        int h_now = 0;
+        auto issue = [&]() {
+            const int slot = op % R::SLOTS;
+            if (!(op & 1)) {
+                if (!more) return;
+                if (ld.s != ids_s || ld.ch >> 3 != ids_b) {
+                    ids_s = ld.s;
+                    ids_b = ld.ch >> 3;
+                    const int p = 32 * ids_b + lane;
+                    ids = p < (st.keys[ids_s] + BKV_BLOCK - 1) / BKV_BLOCK ? (int)A.S.page(ids_s, p, A.L.n_pages) : -1;
+                }
+                page = __shfl_sync(0xffffffffu, ids, 4 * (ld.ch & 7) + c);
+                h_now = ld.h;
+                if (lane < 4) meta[((op >> 1) & (R::META - 1)) * 4 + lane] = page;
+                else page = -1;
+                ld.step(A, st, u_end);
+                more = ld.to_loaded(A, st, u_end);
+            }
+            const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) ptx::mbar_expect_tx(&full[slot], (uint32_t)__popc(there) * R::PAGE);
+            __syncwarp();
+            if (page >= 0) {
+                const int64_t at = ((int64_t)page * A.L.n_kv_head + h_now) * R::PAGE;
+                ptx::bulk_load(mine + slot * R::SLOT + lane * R::STRIDE, (op & 1 ? A.L.v : A.L.k) + at, R::PAGE, &full[slot]);
+            }
+            ++op;
+        };
+#pragma unroll 1
+        for (int i = 0; i < R::SLOTS; ++i) issue();
+        int done = 0;  // half steps consumed
+
+        while (w.u < u_end && ok) {
+            const int s = w.s, h = w.h, tile = w.tile, chunks = w.chunks, c0 = w.ch;
+            const int64_t u0 = w.u - c0;
+            const int c1 = (int)min((int64_t)chunks, c0 + (u_end - w.u));
+            const int n_keys = st.keys[s], n_q = st.n_q[s], first_row = st.first[s];
+            const int c_last = min(c1, w.seen);
+
+            // ---- the tile's query rows as int8 planes, in the order of the K loads
+            uint32_t qa[KW / 2][4];
+            uint32_t qb[KW / 2][SPLIT ? 2 : 4];  // the third plane (SPLIT, 32-bit rows), or the second one of 16 rows
+            float row_fac[NR];  // multiplies a score: scale * log2(e) * the units of the planes
+            int limit[NR];      // keys that the row sees
 #pragma unroll
-        for (int half_row = 0; half_row < NR; ++half_row) {
-            const int r = tile * TR + half_row * 8 + g;
-            const int tok = r / A.group, head = h * A.group + r % A.group;
-            const bool real = tok < n_q;
-            float x[KW * 4];
-            float amax = 0.0f;
-            if (real) {
-                const int64_t at = (int64_t)(first_row + tok) * A.q_ld + (int64_t)head * D;
+            for (int half_row = 0; half_row < NR; ++half_row) {
+                const int r = tile * TR + half_row * 8 + g;
+                const int tok = r / A.group, head = h * A.group + r % A.group;
+                const bool real = tok < n_q;
+                // word i of the lane: 4 channels of the 64-channel part i / 4 (or of what is left behind them)
+                auto channel = [&](int i) { return 64 * (i >> 2) + 4 * ((i >> 2) < KW / 4 ? 4 : KW & 3) * c + 4 * (i & 3); };
+                const int64_t at = (int64_t)(first_row + (real ? tok : 0)) * A.q_ld + (int64_t)head * D;
+                float x[KW][4];
+                if (A.q_f16) {
+                    const __half* p = reinterpret_cast<const __half*>(A.q) + at;
+                    if (A.q_vec) {
+                        uint2 v[KW];
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    // word w of the lane: 4 channels of the 64-channel part w / 4 (or of what is left behind them)
-                    const int part = w >> 2;
-                    constexpr int LEFT = KW & 3;  // words of the last, shorter part
-                    const int words = part < KW / 4 ? 4 : LEFT;
-                    const int d = 64 * part + 4 * words * c + 4 * (w & 3);
-                    if (A.q_f16) {
-                        const __half* p = reinterpret_cast<const __half*>(A.q) + at + d;
-                        if (A.q_vec) {
-                            const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p));
-                            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&v.x));
-                            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&v.y));
-                            x[4 * w] = a.x;
-                            x[4 * w + 1] = a.y;
-                            x[4 * w + 2] = b.x;
-                            x[4 * w + 3] = b.y;
-                        } else {
+                        for (int i = 0; i < KW; ++i) v[i] = __ldcg(reinterpret_cast<const uint2*>(p + channel(i)));
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[4 * w + e] = __half2float(p[e]);
+                        for (int i = 0; i < KW; ++i) {
+                            const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&v[i].x));
+                            const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&v[i].y));
+                            x[i][0] = f0.x;
+                            x[i][1] = f0.y;
+                            x[i][2] = f1.x;
+                            x[i][3] = f1.y;
                         }
                     } else {
-                        const float* p = reinterpret_cast<const float*>(A.q) + at + d;
-                        if (A.q_vec) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4*>(p));
-                            x[4 * w] = v.x;
-                            x[4 * w + 1] = v.y;
-                            x[4 * w + 2] = v.z;
-                            x[4 * w + 3] = v.w;
-                        } else {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) x[4 * w + e] = p[e];
+                        for (int i = 0; i < KW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[i][e] = __half2float(p[channel(i) + e]);
+                    }
+                } else {
+                    const float* p = reinterpret_cast<const float*>(A.q) + at;
+                    if (A.q_vec) {
+#pragma unroll
+                        for (int i = 0; i < KW; ++i) {
+                            const float4 v = __ldcg(reinterpret_cast<const float4*>(p + channel(i)));
+                            x[i][0] = v.x;
+                            x[i][1] = v.y;
+                            x[i][2] = v.z;
+                            x[i][3] = v.w;
                         }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[i][e] = p[channel(i) + e];
                     }
                 }
-            } else {
+                float amax = 0.0f;
+                bool number = true;
 #pragma unroll
-                for (int i = 0; i < KW * 4; ++i) x[i] = 0.0f;
-            }
+                for (int i = 0; i < KW; ++i)
 #pragma unroll
-            for (int i = 0; i < KW * 4; ++i) amax = fmaxf(amax, fabsf(x[i]));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // the row as values below 2 times 2^e: f16 holds it whatever its size
-            uint32_t e = __float_as_uint(amax) & 0x7f800000u;
-            e = e == 0 || e == 0x7f800000u ? 0x3f800000u : min(e, 0x7e800000u);  // zero and infinity stay as they are
-            const float pow2 = __uint_as_float(e), inv2 = __uint_as_float(0x7f000000u - e);
-            row_fac[half_row] = pow2 * (A.scale * L2E);
-            limit[half_row] = real ? max(0, min(n_keys, n_keys - n_q + tok + 1)) : 0;
+                    for (int e = 0; e < 4; ++e) {
+                        amax = fmaxf(amax, fabsf(x[i][e]));
+                        number &= x[i][e] == x[i][e];
+                    }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                number = (__ballot_sync(0xffffffffu, number) >> (4 * g) & 15) == 15;
+                // planes: q = amax / 127 * (p1 + p2 / 254 + p3 / 254^2). Two of them hold it to 2^-16 of the row's
+                // largest, three to 2^-24. Below 1e-35 a row's products with any scale count as zero.
+                const float unit = amax > 1e-35f ? 127.0f / amax : 0.0f;
+                row_fac[half_row] = number && amax < INFINITY ? amax * (1.0f / (127.0f * (P3 ? 64516.0f : 254.0f))) * (A.scale * L2E)
+                                                              : __uint_as_float(0x7fc00000u);
+                limit[half_row] = real ? max(0, min(n_keys, n_keys - n_q + tok + 1)) : 0;
 #pragma unroll
-            for (int w = 0; w < KW; ++w) {
-                const float y0 = x[4 * w] * inv2, y1 = x[4 * w + 1] * inv2, y2 = x[4 * w + 2] * inv2, y3 = x[4 * w + 3] * inv2;
-                const uint32_t h0 = pack_f16(y0, y1), h1 = pack_f16(y2, y3);
-                if constexpr (SPLIT) {
-                    qa[w][0] = h0;
-                    qa[w][1] = pack_rest(y0, y1, h0);
-                    qa[w][2] = h1;
-                    qa[w][3] = pack_rest(y2, y3, h1);
-                } else {
-                    qa[w][half_row] = h0;
-                    qa[w][2 + half_row] = h1;
-                }
-            }
-        }
-
-        float m[NR], l[NR];
-        float o[NT][4];
-        float frame = __uint_as_float(0x00800000u);  // power of two at or above half of every V scale so far
+                for (int i = 0; i < KW; ++i) {
+                    float y[4];
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-
-        // no row of the tile sees a key from here on
-        int seen = limit[0];
-        if constexpr (NR == 2) seen = max(seen, limit[1]);
-        seen = __reduce_max_sync(0xffffffffu, seen);
-        const int c_last = min(c1, (seen + 63) / 64);
-
-        int64_t next_page = c0 < c_last ? A.S.page(s, 4 * c0 + c, A.L.n_pages) : -1;
-        for (int ch = c0; ch < c_last; ++ch) {
-            const int64_t page = next_page;
-            if (ch + 1 < c_last) next_page = A.S.page(s, 4 * (ch + 1) + c, A.L.n_pages);
-            const bool there = page >= 0 && 64 * ch + 16 * c < seen;  // a page behind the last seen key may hold anything
-            const int64_t head_at = (there ? page : 0) * A.L.n_kv_head + h;
-            const int64_t k_head = __shfl_sync(0xffffffffu, head_at, g >> 1);  // lane g / 2 holds page g / 2
-            const int8_t* kp = A.L.k + k_head * (BKV_BLOCK * D) + (g & 1) * D;
-            const int8_t* vp = A.L.v + head_at * (BKV_BLOCK * D) + g * BKV_BLOCK;
-            const float ks = there ? A.L.ks[head_at] : 0.0f;
-            const float vs = there ? A.L.vs[head_at] : 0.0f;
-
-            // ---- scores
-            float sc[8][4];
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) sc[t][e] = 0.0f;
-                uint32_t kw[KW];
-#pragma unroll
-                for (int part = 0; part < KW / 4; ++part) {
-                    const uint4 v4 = __ldcg(reinterpret_cast<const uint4*>(kp + 2 * t * D + 64 * part + 16 * c));
-                    kw[4 * part] = v4.x;
-                    kw[4 * part + 1] = v4.y;
-                    kw[4 * part + 2] = v4.z;
-                    kw[4 * part + 3] = v4.w;
-                }
-                if constexpr ((KW & 3) == 2) {
-                    const uint2 v2 = __ldcg(reinterpret_cast<const uint2*>(kp + 2 * t * D + 64 * (KW / 4) + 8 * c));
-                    kw[KW - 2] = v2.x;
-                    kw[KW - 1] = v2.y;
-                }
-#pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    uint32_t b0, b1;
-                    s8x4_to_f16(kw[w], b0, b1);
-                    mma16816(sc[t], qa[w][0], qa[w][1], qa[w][2], qa[w][3], b0, b1);
+                    for (int e = 0; e < 4; ++e) y[e] = x[i][e] * unit;
+                    const uint32_t p1 = take_plane(y), p2 = take_plane(y);
+                    const int a = 2 * (i & 1);
+                    if constexpr (SPLIT) {
+                        qa[i / 2][a] = p1;
+                        qa[i / 2][a + 1] = p2;
+                        qb[i / 2][i & 1] = P3 ? take_plane(y) : 0;
+                    } else {
+                        qa[i / 2][a + half_row] = p1;
+                        qb[i / 2][a + half_row] = p2;
+                    }
                 }
             }
 
-            // ---- softmax step. Lane c holds tokens 0..15 of page 4 ch + c: x[row][token]
-            const int key0 = 64 * ch + 16 * c;
-            float w_scale;
-            float corr_o[NR];
-            float x[NR][16];
-            {
-                // the V scales' frame
-                float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
-                vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-                const float pow2 = fmaxf(frame, __uint_as_float(__float_as_uint(vmax) & 0x7f800000u));
-                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(pow2));
-                w_scale = vs * inv;
-#pragma unroll
-                for (int i = 0; i < NR; ++i) corr_o[i] = frame * inv;
-                frame = pow2;
-            }
+            float m[NR], l[NR];
+            float o[NT][4];
+            float frame = __uint_as_float(0x00800000u);  // power of two at or above half of every V scale so far
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
-                const float f = ks * row_fac[i];
-                float mx = -INFINITY;
+                m[i] = -INFINITY;
+                l[i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+
+            for (int ch = c0; ch < c_last; ++ch) {
+                // ---- scores
+                int slot = done % R::SLOTS;
+                if (!ptx::mbar_wait(&full[slot], (done / R::SLOTS) & 1)) {
+                    ok = false;
+                    break;
+                }
+                const int id = meta[((done >> 1) & (R::META - 1)) * 4 + c];  // this lane's page
+                const bool there = id >= 0;
+                float ks = 0.0f, vs = 0.0f;
+                if (there) {
+                    const int64_t at = (int64_t)id * A.L.n_kv_head + h;
+                    ks = __ldcg(A.L.ks + at);
+                    vs = __ldcg(A.L.vs + at);
+                }
+                const uint8_t* kp = mine + slot * R::SLOT + (g >> 1) * R::STRIDE + (g & 1) * D;
+                int sc[8][4], sd[8][P3 || !SPLIT ? 4 : 1];
 #pragma unroll
                 for (int t = 0; t < 8; ++t)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float y = SPLIT ? sc[t][e] + sc[t][2 + e] : sc[t][2 * i + e];
-                        y *= f;
-                        if (!there || key0 + 2 * t + e >= limit[i]) y = -INFINITY;
-                        x[i][2 * t + e] = y;
-                        mx = fmaxf(mx, y);
+                    for (int e = 0; e < 4; ++e) {
+                        sc[t][e] = 0;
+                        if constexpr (P3 || !SPLIT) sd[t][e] = 0;
                     }
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float m_new = fmaxf(m[i], mx);
-                const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-                const float corr = ex2(m[i] - m_use);
-                m[i] = m_new;
-                float sum = 0.0f;
+                // four tiles side by side, so that independent products are under way
 #pragma unroll
-                for (int t = 0; t < 16; ++t) {
-                    x[i][t] = ex2(x[i][t] - m_use);
-                    sum += x[i][t];
+                for (int t0 = 0; t0 < 8; t0 += 4)
+#pragma unroll
+                    for (int part = 0; part < (KW + 3) / 4; ++part) {
+                        uint32_t kw[4][4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const uint8_t* at = kp + 2 * (t0 + t) * D + 64 * part;
+                            if (part < KW / 4) {
+                                const uint4 v4 = *reinterpret_cast<const uint4*>(at + 16 * c);
+                                kw[t][0] = v4.x;
+                                kw[t][1] = v4.y;
+                                kw[t][2] = v4.z;
+                                kw[t][3] = v4.w;
+                            } else {
+                                const uint2 v2 = *reinterpret_cast<const uint2*>(at + 8 * c);
+                                kw[t][0] = v2.x;
+                                kw[t][1] = v2.y;
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < (part < KW / 4 ? 2 : 1); ++i)
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const uint32_t* qf = qa[2 * part + i];
+                                const uint32_t* qg = qb[2 * part + i];
+                                mma16832(sc[t0 + t], qf[0], qf[1], qf[2], qf[3], kw[t][2 * i], kw[t][2 * i + 1]);
+                                if constexpr (!SPLIT) mma16832(sd[t0 + t], qg[0], qg[1], qg[2], qg[3], kw[t][2 * i], kw[t][2 * i + 1]);
+                                else if constexpr (P3) mma16832(sd[t0 + t], qg[0], 0, qg[1], 0, kw[t][2 * i], kw[t][2 * i + 1]);
+                            }
+                    }
+                __syncwarp();
+                ++done;
+                issue();  // into the slot that has just been read
+
+                // ---- softmax step. Lane c holds tokens 0..15 of page 4 ch + c: x[row][token]
+                const int key0 = 64 * ch + 16 * c;
+                float w_scale;
+                float corr_o[NR];
+                float x[NR][16];
+                {
+                    // the V scales' frame
+                    float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
+                    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
+                    const float pow2 = fmaxf(frame, __uint_as_float(__float_as_uint(vmax) & 0x7f800000u));
+                    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(pow2));
+                    w_scale = vs * inv;
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) corr_o[i] = frame * inv;
+                    frame = pow2;
                 }
-                l[i] = fmaf(l[i], corr, sum);
-                corr_o[i] *= corr;
-            }
-            bool turn = corr_o[0] != 1.0f;
-            if constexpr (NR == 2) turn |= corr_o[1] != 1.0f;
-            if (__any_sync(0xffffffffu, turn)) {
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    o[i][0] *= corr_o[0];
-                    o[i][1] *= corr_o[0];
-                    o[i][2] *= corr_o[NR - 1];
-                    o[i][3] *= corr_o[NR - 1];
-                }
-            }
-            // ---- weights as f16 operands: k step t' holds tokens 4t' .. 4t' + 3 of each lane's page
-            uint32_t pa[4][4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
-                    const float y0 = x[i][4 * t] * w_scale, y1 = x[i][4 * t + 1] * w_scale, y2 = x[i][4 * t + 2] * w_scale,
-                                y3 = x[i][4 * t + 3] * w_scale;
-                    const uint32_t h0 = pack_f16(y0, y1), h1 = pack_f16(y2, y3);
-                    if constexpr (SPLIT) {
-                        pa[t][0] = h0;
-                        pa[t][1] = pack_rest(y0, y1, h0);
-                        pa[t][2] = h1;
-                        pa[t][3] = pack_rest(y2, y3, h1);
-                    } else {
-                        pa[t][i] = h0;
-                        pa[t][2 + i] = h1;
+                        const float f = fmaxf(ks * row_fac[i], 1e-37f);  // above 0: a masked token's -inf stays -inf
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 8; ++t)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            // |p1 . k| <= 127 * 127 * 256: 254 of them fit 32 bits
+                            float y;
+                            if constexpr (!SPLIT) y = (float)(sc[t][2 * i + e] * 254 + sd[t][2 * i + e]);
+                            else if constexpr (P3) y = fmaf((float)(sc[t][e] * 254 + sc[t][2 + e]), 254.0f, (float)sd[t][e]);
+                            else y = (float)(sc[t][e] * 254 + sc[t][2 + e]);
+                            x[i][2 * t + e] = y;
+                        }
+                    const int left = there ? limit[i] - key0 : 0;  // of the lane's tokens the row sees the first `left`
+                    if (__any_sync(0xffffffffu, left < 16)) {
+#pragma unroll
+                        for (int t = 0; t < 16; ++t)
+                            if (t >= left) x[i][t] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) mx = fmaxf(mx, x[i][t]);
+                    mx *= f;
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    const float m_new = fmaxf(m[i], mx);
+                    const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                    const float corr = ex2(m[i] - m_use);
+                    m[i] = m_new;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int t = 0; t < 16; ++t) {
+                        x[i][t] = ex2(fmaf(x[i][t], f, -m_use));
+                        sum += x[i][t];
+                    }
+                    l[i] = fmaf(l[i], corr, sum);
+                    corr_o[i] *= corr;
+                }
+                bool turn = corr_o[0] != 1.0f;
+                if constexpr (NR == 2) turn |= corr_o[1] != 1.0f;
+                if (__any_sync(0xffffffffu, turn)) {
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        o[i][0] *= corr_o[0];
+                        o[i][1] *= corr_o[0];
+                        o[i][2] *= corr_o[NR - 1];
+                        o[i][3] *= corr_o[NR - 1];
                     }
                 }
-            }
-            // ---- O += P.V
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const uint4 v4 = __ldcg(reinterpret_cast<const uint4*>(vp + 8 * i * BKV_BLOCK));
-                const uint32_t vw[4] = {v4.x, v4.y, v4.z, v4.w};
+                // ---- weights as f16 operands: k step t holds tokens 4t .. 4t + 3 of each lane's page
+                uint32_t pa[4][4];
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
-                    uint32_t b0, b1;
-                    s8x4_to_f16(vw[t], b0, b1);
-                    mma16816(o[i], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b0, b1);
+#pragma unroll
+                    for (int i = 0; i < NR; ++i) {
+                        const float y0 = x[i][4 * t] * w_scale, y1 = x[i][4 * t + 1] * w_scale, y2 = x[i][4 * t + 2] * w_scale,
+                                    y3 = x[i][4 * t + 3] * w_scale;
+                        const uint32_t h0 = pack_f16(y0, y1), h1 = pack_f16(y2, y3);
+                        if constexpr (SPLIT) {
+                            pa[t][0] = h0;
+                            pa[t][1] = pack_rest(y0, y1, h0);
+                            pa[t][2] = h1;
+                            pa[t][3] = pack_rest(y2, y3, h1);
+                        } else {
+                            pa[t][i] = h0;
+                            pa[t][2 + i] = h1;
+                        }
+                    }
                 }
+                // ---- O += P.V
+                slot = done % R::SLOTS;
+                if (!ptx::mbar_wait(&full[slot], (done / R::SLOTS) & 1)) {
+                    ok = false;
+                    break;
+                }
+                const uint8_t* vp = mine + slot * R::SLOT + c * R::STRIDE + g * BKV_BLOCK;
+#pragma unroll
+                for (int i0 = 0; i0 < NT; i0 += 4) {
+                    uint32_t vw[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 v4 = *reinterpret_cast<const uint4*>(vp + 8 * (i0 + i) * BKV_BLOCK);
+                        vw[i][0] = v4.x;
+                        vw[i][1] = v4.y;
+                        vw[i][2] = v4.z;
+                        vw[i][3] = v4.w;
+                    }
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t b0, b1;
+                            s8x4_to_f16(vw[i][t], b0, b1);
+                            mma16816(o[i0 + i], pa[t][0], pa[t][1], pa[t][2], pa[t][3], b0, b1);
+                        }
+                }
+                __syncwarp();
+                ++done;
+                issue();
             }
-        }
 
-        // ---- the item's rows: finished, or left for the combine kernel
+            // ---- the item's rows: finished, or a part of them
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-        }
-        const bool alone = c0 == 0 && c1 == chunks;
-        const int64_t slot = me * 2 + (u == u_begin ? 0 : 1);
-        if (!alone && c0 == 0 && lane == 0) A.todo[me] = 
-            make_int4(s, h, tile, (int)((u + chunks - 1) / per - me) * 2 + (u == u_begin ? 0 : 1));
+            for (int i = 0; i < NR; ++i) {
+                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+                l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            }
+            const bool alone = c0 == 0 && c1 == chunks;
+            const int which = w.u == u_begin ? 0 : 1;
+            const int64_t part = ((int64_t)blockIdx.x * AW + warp) * 2 + which;
+            if (!alone && lane == 0) parts[2 * warp + which] = Part{u0, chunks, s, h, tile, warp == 0 || c0 == 0};
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int r = tile * TR + i * 8 + g;
-            const int tok = r / A.group, head = h * A.group + r % A.group;
-            if (tok >= n_q) continue;
-            const float fin = alone ? (l[i] > 0.0f ? frame / l[i] : 0.0f) : frame;
-            const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
-            float* po = A.part_o + (slot * TR + i * 8 + g) * D + 2 * c;
-            if (!alone && c == 0) A.part_ml[slot * TR + i * 8 + g] = make_float2(m[i], l[i]);
+            for (int i = 0; i < NR; ++i) {
+                const int r = tile * TR + i * 8 + g;
+                const int tok = r / A.group, head = h * A.group + r % A.group;
+                if (tok >= n_q) continue;
+                const float fin = alone ? (l[i] > 0.0f ? frame / l[i] : 0.0f) : frame;
+                const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
+                float* po = A.warp_o + (part * TR + i * 8 + g) * D + 2 * c;
+                if (!alone && c == 0) A.warp_ml[part * TR + i * 8 + g] = make_float2(m[i], l[i]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                float y0, y1;
-                if constexpr (SPLIT) {
-                    y0 = (o[n][0] + o[n][2]) * fin;
-                    y1 = (o[n][1] + o[n][3]) * fin;
-                } else {
-                    y0 = o[n][2 * i] * fin;
-                    y1 = o[n][2 * i + 1] * fin;
-                }
-                if (!alone) {
-                    *reinterpret_cast<float2*>(po + 8 * n) = make_float2(y0, y1);
-                } else if (A.out_f16) {
-                    __half* p = reinterpret_cast<__half*>(A.out) + at + 8 * n;
-                    p[0] = __float2half_rn(y0);
-                    p[1] = __float2half_rn(y1);
-                } else {
-                    float* p = reinterpret_cast<float*>(A.out) + at + 8 * n;
-                    p[0] = y0;
-                    p[1] = y1;
+                for (int n = 0; n < NT; ++n) {
+                    float y0, y1;
+                    if constexpr (SPLIT) {
+                        y0 = (o[n][0] + o[n][2]) * fin;
+                        y1 = (o[n][1] + o[n][3]) * fin;
+                    } else {
+                        y0 = o[n][2 * i] * fin;
+                        y1 = o[n][2 * i + 1] * fin;
+                    }
+                    if (alone) store_pair(A, at + 8 * n, y0, y1);
+                    else *reinterpret_cast<float2*>(po + 8 * n) = make_float2(y0, y1);
                 }
             }
+            w.u += c1 - c0;
+            w.ch = c1;
+            if (c1 == chunks) w.next_item(A, st, u_end);
         }
-        u += c1 - c0;
+        // a wait that gave up: the copies still under way end before the block does
+        for (int i = done; !ok && i < op; ++i) ptx::mbar_wait(&full[i % R::SLOTS], (i / R::SLOTS) & 1);
+    }
+    if (!ok && lane == 0) atomicExch(A.err, 1);
+    __syncthreads();
+
+    // ---- parts of one item within the block, then what the block shares with others
+    // lane i: whether part i is the block's first one of its item (the second part of a warp starts its item)
+    const unsigned heads = __ballot_sync(
+        0xffffffffu, lane < 2 * AW && parts[min(lane, 2 * AW - 1)].chunks && parts[min(lane, 2 * AW - 1)].head);
+    static_assert(2 * AW <= 32, "a lane for each part");
+    Part open[2];
+    int n_open = 0;
+    int job = warp;
+    for (unsigned left = heads; left; left &= left - 1) {  // the rows of all items in turn, one warp each
+        const int i = __ffs(left) - 1;
+        const Part p = parts[i];
+        const bool whole = p.u0 >= block_begin && p.u0 + p.chunks <= block_end;
+        if (!whole) open[n_open++] = p;
+        const int rows = min(TR, st.n_q[p.s] * A.group - p.tile * TR);
+        if (job < rows) {
+            int n = 1;  // the warps behind the first one have their part of the item at the start of their range
+            while (i / 2 + n < AW && parts[2 * (i / 2 + n)].chunks && parts[2 * (i / 2 + n)].u0 == p.u0) ++n;
+            const int64_t to = ((int64_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * TR;
+            auto nth = [&](int j) { return ((int64_t)blockIdx.x * AW * 2 + (j ? 2 * (i / 2 + j) : i)) * TR; };
+            for (; job < rows; job += AW)
+                join_row<D>(A, n, job, st.first[p.s], p.tile * TR, p.h, [&](int j) { return A.warp_o + nth(j) * D; },
+                            [&](int j) { return A.warp_ml + nth(j); }, whole ? nullptr : A.block_o + to * D,
+                            whole ? nullptr : A.block_ml + to);
+        }
+        job -= rows;
+    }
+    if (n_open == 0) return;
+    auto block_of = [&](int64_t u) { return (int)(((u + 1) * n_block + total - 1) / total) - 1; };  // whose share has step u
+    __syncthreads();
+    if (threadIdx.x < n_open) {
+        const Part p = open[threadIdx.x];
+        const int first = block_of(p.u0), n = block_of(p.u0 + p.chunks - 1) - first + 1;
+        __threadfence();  // the block's parts, written before the barrier, come before its arrival
+        const unsigned before = atomicAdd(&A.arrived[first], 1u);
+        last_one[threadIdx.x] = before == (unsigned)n - 1;
+        if (before == (unsigned)n - 1) A.arrived[first] = 0;  // at rest again
+        __threadfence();
+    }
+    __syncthreads();
+    for (int k = 0; k < n_open; ++k) {
+        if (!last_one[k]) continue;
+        const Part p = open[k];
+        const int64_t first = block_of(p.u0);
+        const int n = block_of(p.u0 + p.chunks - 1) - (int)first + 1;
+        const int rows = min(TR, st.n_q[p.s] * A.group - p.tile * TR);
+        // the item starts somewhere in its first block's range, and at the start of every other one's
+        auto nth = [&](int b) { return ((first + b) * 2 + (b == 0 && p.u0 != first * total / n_block ? 1 : 0)) * TR; };
+        for (int r = warp; r < rows; r += AW)
+            join_row<D>(A, n, r, st.first[p.s], p.tile * TR, p.h, [&](int b) { return A.block_o + nth(b) * D; },
+                        [&](int b) { return A.block_ml + nth(b); }, nullptr, nullptr);
     }
 }
 
-// Joins the parts of one item that several warps of the attention shared: block
-// b has the item that starts in warp b's range. A warp takes a row at a time.
-constexpr int CW = 8;
-template <int D, bool SPLIT>
-__global__ void __launch_bounds__(32 * CW) bkv_combine_kernel(AttnArgs A) {
-    pdl_entry();
-    constexpr int TR = SPLIT ? 8 : 16;
-    constexpr int V = D / 32;  // channels of a lane
-    const int64_t w0 = blockIdx.x;
-    const int4 t = A.todo[w0];
-    if (t.x < 0) return;
-    const int s = t.x, h = t.y, tile = t.z, last = t.w >> 1;  // the parts of warps w0 .. w0 + last
-    int first_row, n_q;
-    A.S.rows(s, first_row, n_q);
-    __shared__ float so[CW][D];
-    __shared__ float2 sml[CW];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int r = 0; r < TR; ++r) {
-        const int row = tile * TR + r, tok = row / A.group, head = h * A.group + row % A.group;
-        if (tok >= n_q) break;
-        float m = -INFINITY, l = 0.0f, acc[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-        for (int p = warp; p <= last; p += CW) {
-            const int64_t slot = (w0 + p) * 2 + (p == 0 ? t.w & 1 : 0);  // a later part starts its warp's range
-            const float2 ml = __ldcg(&A.part_ml[slot * TR + r]);
-            const float* po = A.part_o + (slot * TR + r) * D + lane;
-            float y[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) y[i] = __ldcg(po + 32 * i);
-            if (ml.x == -INFINITY) continue;
-            const float m_new = fmaxf(m, ml.x);
-            const float a = ex2(m - m_new), b = ex2(ml.x - m_new);
-            l = l * a + ml.y * b;
-#pragma unroll
-            for (int i = 0; i < V; ++i) acc[i] = acc[i] * a + y[i] * b;
-            m = m_new;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) so[warp][lane + 32 * i] = acc[i];
-        if (lane == 0) sml[warp] = make_float2(m, l);
-        __syncthreads();
-        for (int d = threadIdx.x; d < D; d += blockDim.x) {
-            float M = -INFINITY, Lr = 0.0f, O = 0.0f;
-            for (int w = 0; w < CW; ++w) M = fmaxf(M, sml[w].x);
-            for (int w = 0; w < CW; ++w) {
-                if (sml[w].x == -INFINITY) continue;
-                const float f = ex2(sml[w].x - M);
-                Lr += sml[w].y * f;
-                O += so[w][d] * f;
-            }
-            const float y = Lr > 0.0f ? O / Lr : 0.0f;
-            const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + d;
-            if (A.out_f16) reinterpret_cast<__half*>(A.out)[at] = __float2half_rn(y);
-            else reinterpret_cast<float*>(A.out)[at] = y;
-        }
-        __syncthreads();
-    }
-}
-
-template <int D, bool SPLIT>
+template <int D, bool SPLIT, bool P3>
 void launch_attn(vkb_context* ctx, AttnArgs A) {
-    constexpr int TR = SPLIT ? 8 : 16;
-    const unsigned blocks = (unsigned)(ctx->sm_count * (D <= 64 ? 3 : D <= 128 ? 2 : 1));
-    const size_t warps = (size_t)blocks * AW;
-    const size_t o_bytes = warps * 2 * TR * D * sizeof(float), ml_bytes = warps * 2 * TR * sizeof(float2);
-    ctx->ensure_workspace(o_bytes + ml_bytes + warps * sizeof(int4));
+    constexpr int TR = SPLIT ? 8 : 16, AW = Ring<D>::AW;
+    constexpr int SMEM = ((int)sizeof(Streams) + 15) / 16 * 16 + AW * Ring<D>::WARP_BYTES;
+    static_assert(SMEM <= 227 * 1024 - 2048, "shared memory of one block");
+    const size_t blocks = (size_t)ctx->sm_count;
+    const size_t warp_o = blocks * AW * 2 * TR * D * sizeof(float), block_o = blocks * 2 * TR * D * sizeof(float);
+    const size_t warp_ml = blocks * AW * 2 * TR * sizeof(float2), block_ml = blocks * 2 * TR * sizeof(float2);
+    ctx->ensure_workspace(warp_o + block_o + warp_ml + block_ml);
     uint8_t* ws = ctx->workspace.as<uint8_t>();
-    A.part_o = reinterpret_cast<float*>(ws);
-    A.part_ml = reinterpret_cast<float2*>(ws + o_bytes);
-    A.todo = reinterpret_cast<int4*>(ws + o_bytes + ml_bytes);
-    const size_t smem = (size_t)(A.S.n_seq + 1) * sizeof(int64_t);
-    auto kern = bkv_attn_kernel<D, SPLIT>;
-    if (smem > 40 * 1024) smem_optin(kern, 72 * 1024);
-    launch_pdl(ctx, kern, dim3(blocks), 32 * AW, smem, A);
-    VKB_CUDA(cudaGetLastError());
-    ctx->count();
-    launch_pdl(ctx, bkv_combine_kernel<D, SPLIT>, dim3((unsigned)warps), 32 * CW, 0, A);
-    VKB_CUDA(cudaGetLastError());
-    ctx->count();
+    A.warp_o = reinterpret_cast<float*>(ws);
+    A.block_o = reinterpret_cast<float*>(ws + warp_o);
+    A.warp_ml = reinterpret_cast<float2*>(ws + warp_o + block_o);
+    A.block_ml = reinterpret_cast<float2*>(ws + warp_o + block_o + warp_ml);
+    A.arrived = ctx->tile_ctr.as<unsigned>();
+    A.err = ctx->err_flag.as<int>();
+    auto kern = bkv_attn_kernel<D, SPLIT, P3>;
+    smem_optin(kern, SMEM);
+    const BkvStreams all = A.S;
+    for (int s0 = 0; s0 < all.n_seq; s0 += BKV_SEQ_PER_LAUNCH) {
+        A.S.n_seq = std::min(all.n_seq - s0, BKV_SEQ_PER_LAUNCH);
+        A.S.start = all.start + s0;
+        A.S.len = all.len + s0;
+        A.S.table = all.table + (int64_t)s0 * all.ld;
+        launch_pdl(ctx, kern, dim3((unsigned)blocks), 32 * AW, SMEM, A);
+        VKB_CUDA(cudaGetLastError());
+        ctx->count();
+    }
 }
 
 }  // namespace
@@ -556,14 +848,15 @@ extern "C" vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* c
         A.q = q_dev;
         A.q_ld = q_ld;
         A.q_vec = (uintptr_t)q_dev % (A.q_f16 ? 8 : 16) == 0 && q_ld % 4 == 0;
+        A.out_vec = (uintptr_t)out_dev % (A.out_f16 ? 4 : 8) == 0 && out_ld % 2 == 0;
         A.scale = scale;
         A.out = out_dev;
         A.out_ld = out_ld;
         NvtxRange nvtx_range("vkb.bkv.attention");
-        const bool split = !A.q_f16 || !A.out_f16 || (int64_t)batch->max_q * A.group <= 8;
         with_bkv_head(cache->d_head, [&](auto D) {
-            if (split) launch_attn<decltype(D)::value, true>(ctx, A);
-            else launch_attn<decltype(D)::value, false>(ctx, A);
+            if (!A.q_f16 || !A.out_f16) launch_attn<decltype(D)::value, true, true>(ctx, A);
+            else if ((int64_t)batch->max_q * A.group <= 8) launch_attn<decltype(D)::value, true, false>(ctx, A);
+            else launch_attn<decltype(D)::value, false, false>(ctx, A);
         });
     });
 }
