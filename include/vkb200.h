@@ -528,7 +528,8 @@ typedef struct vkb_bkv_cache {
  * position kv_len[s] - 1. Page p of the stream is table[s * table_ld + p]; an id
  * outside 0..n_pages-1 is a page that is not there: it is never written, and
  * its tokens are not seen. n_tok = tok_start[n_seq]; max_q is the largest
- * number of rows of one stream (a hint for the launch: a wrong one costs time). */
+ * number of rows of one stream (a hint for the choice of kernels: a wrong one
+ * costs time). */
 typedef struct vkb_bkv_batch {
     int32_t n_seq, n_tok, max_q;
     const int32_t* tok_start_dev;  /* [n_seq + 1] */
@@ -555,7 +556,8 @@ VKB_API vkb_status vkb_bkv_append(vkb_context* ctx, const vkb_bkv_cache* cache, 
  * [n_tok] rows of n_head*d_head values, row strides in elements, F32 or F16
  * each. With an F32 q or out the products are accurate to about 2^-21, else
  * q and the weights enter them as f16; sums and statistics are fp32 either
- * way. A row without keys (a stream of length 0) is zero. */
+ * way. A row without keys (a stream of length 0) is zero; a row of q with an
+ * infinity or NaN is NaN. */
 VKB_API vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,
                                      const vkb_bkv_batch* batch, int32_t n_head, const void* q_dev, int64_t q_ld,
                                      int32_t q_dtype, float scale, void* out_dev, int64_t out_ld, int32_t out_dtype);

@@ -295,6 +295,57 @@ def test_prompt_chunks(ctx, d, dtype, new, lens):
     check_attention(ctx, rng, lens, new, 2, 2, d, dtype)
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,group,new,lens", [
+    (8, 4, [300, 1, 129, 0, 64], [300, 700, 1000, 50, 64]),    # tiles that end inside 128 and 256 rows, streams with few rows between
+    (16, 1, [600, 513], [640, 4000]),
+    (16, 3, [256, 100, 90], [255, 100, 91]),                   # more rows than tokens: rows without any key
+])
+def test_many_rows_of_16_bits(ctx, d, heads, group, new, lens):
+    """Enough row tiles for the tensor-core kernel; against the kernel for few rows, which 32-bit rows take, and 64 bits on some heads."""
+    import torch
+    rng = np.random.default_rng(d + heads + group)
+    start = np.concatenate([[0], np.cumsum(new)])
+    table, n_pages = tables(rng, lens, missing=[(1, 2)])
+    plain = filled(rng, n_pages, heads, d)
+    plain.vs[rng.random(plain.vs.shape) < 0.2] *= np.float32(40)     # V scales rise along the way
+    plain.vs /= np.float32(40)
+    cache = cache_of(ctx, plain)
+    b = batch_of(table, start, lens)
+    q = rng.standard_normal((start[-1], heads * group, d)).astype(np.float16)
+    got = cache.attention(0, b, dev(q), scale=d ** -0.5)
+    few = cache.attention(0, b, dev(q.astype(np.float32)), scale=d ** -0.5)
+    assert torch.isfinite(got).all()
+    assert float((got.float() - few).abs().max()) <= TOL["float16"]
+    sub = Plain(n_pages, 1, d)
+    h = heads - 1
+    sub.k, sub.v, sub.ks, sub.vs = plain.k[:, h:h + 1], plain.v[:, h:h + 1], plain.ks[:, h:h + 1], plain.vs[:, h:h + 1]
+    want = sub.attention(table, start, lens, q[:, h * group:(h + 1) * group], d ** -0.5)
+    assert np.max(np.abs(got[:, h * group:(h + 1) * group].cpu().numpy() - want)) <= TOL["float16"]
+    again = cache.attention(0, b, dev(q), scale=d ** -0.5)
+    assert torch.equal(got, again)
+
+
+def test_rows_that_are_not_numbers(ctx):
+    """A row of q with NaN or an infinity is NaN; the others are as they would be."""
+    rng = np.random.default_rng(19)
+    for dtype, heads, group, new in (("float32", 2, 2, [3, 1]), ("float16", 2, 2, [2, 1]), ("float16", 2, 8, [3, 2]), ("float16", 16, 4, [300, 200])):
+        lens = [n + 70 for n in new]
+        start = np.concatenate([[0], np.cumsum(new)])
+        table, n_pages = tables(rng, lens)
+        cache = cache_of(ctx, filled(rng, n_pages, heads, 64))
+        b = batch_of(table, start, lens)
+        q = rng.standard_normal((start[-1], heads * group, 64)).astype(dtype)
+        want = cache.attention(0, b, dev(q)).cpu().numpy()
+        bad = np.zeros(q.shape[:2], bool)
+        for i, (r, h, x) in enumerate([(0, 0, np.nan), (0, 3, np.inf), (start[-1] - 1, 1, -np.inf), (1, 2, np.nan)]):
+            q[r, h, 7 * i] = x
+            bad[r, h] = True
+        got = cache.attention(0, b, dev(q)).cpu().numpy()
+        assert np.isnan(got[bad]).all()
+        assert np.array_equal(got[~bad], want[~bad])
+
+
 @pytest.mark.parametrize("dtype", ["float32", "float16"])
 def test_one_long_stream_and_many_short_ones(ctx, dtype):
     rng = np.random.default_rng(11)

@@ -32,7 +32,7 @@
 // ragged lengths balance themselves. A warp finishes an item that lies in its
 // share alone; parts of shared items are joined in order, first within the
 // block, then by the last block of the item to arrive.
-#include "bkv.cuh"
+#include "bkv_attn.cuh"
 #include "tc_ptx.cuh"
 #include <algorithm>
 
@@ -95,16 +95,8 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
     return pack_f16(a - h.x, b - h.y);
 }
 
-struct AttnArgs {
-    BkvLayer L;
-    BkvStreams S;
-    int group, n_head;
-    const void* q;
-    int64_t q_ld;
-    float scale;
-    void* out;
-    int64_t out_ld;
-    int q_f16, out_f16, q_vec, out_vec;
+struct AttnArgs : BkvAttn {
+    int q_vec, out_vec;
     float* warp_o;    // [blocks * AW][2][rows][D]: a warp's parts of items that it shares with others
     float2* warp_ml;  // [blocks * AW][2][rows]
     float* block_o;   // [blocks][2][rows][D]: the same of a block
@@ -315,7 +307,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& A, int n, int r, int64_
         if (lane == 0) to_ml[r] = make_float2(m, l);
     } else {
         const int row = tile_row0 + r, tok = row / A.group, head = h * A.group + row % A.group;
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         const int64_t at = (row_at + tok) * A.out_ld + (int64_t)head * D;
 #pragma unroll
         for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
@@ -591,7 +583,8 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 }
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
-                        const float f = fmaxf(ks * row_fac[i], 1e-37f);  // above 0: a masked token's -inf stays -inf
+                        float f = ks * row_fac[i];
+                    if (f < 1e-37f) f = 1e-37f;  // above 0: a masked token's -inf stays -inf (and NaN stays NaN)
                     float mx = -INFINITY;
 #pragma unroll
                     for (int t = 0; t < 8; ++t)
@@ -706,7 +699,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 const int r = tile * TR + i * 8 + g;
                 const int tok = r / A.group, head = h * A.group + r % A.group;
                 if (tok >= n_q) continue;
-                const float fin = alone ? (l[i] > 0.0f ? frame / l[i] : 0.0f) : frame;
+                const float fin = alone ? (l[i] == 0.0f ? 0.0f : frame / l[i]) : frame;
                 const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
                 float* po = A.warp_o + (part * TR + i * 8 + g) * D + 2 * c;
                 if (!alone && c == 0) A.warp_ml[part * TR + i * 8 + g] = make_float2(m[i], l[i]);
@@ -818,6 +811,19 @@ void launch_attn(vkb_context* ctx, AttnArgs A) {
 }
 
 }  // namespace
+
+void run_bkv_attn(vkb_context* ctx, const BkvAttn& a) {
+    AttnArgs A{};
+    static_cast<BkvAttn&>(A) = a;
+    A.q_vec = (uintptr_t)a.q % (a.q_f16 ? 8 : 16) == 0 && a.q_ld % 4 == 0;
+    A.out_vec = (uintptr_t)a.out % (a.out_f16 ? 4 : 8) == 0 && a.out_ld % 2 == 0;
+    with_bkv_head(a.d_head, [&](auto D) {
+        if (!a.q_f16 || !a.out_f16) launch_attn<decltype(D)::value, true, true>(ctx, A);
+        else if ((int64_t)a.max_q * a.group <= 8) launch_attn<decltype(D)::value, true, false>(ctx, A);
+        else launch_attn<decltype(D)::value, false, false>(ctx, A);
+    });
+}
+
 }  // namespace vkb
 
 using namespace vkb;
@@ -826,37 +832,34 @@ extern "C" vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* c
                                         const vkb_bkv_batch* batch, int32_t n_head, const void* q_dev, int64_t q_ld,
                                         int32_t q_dtype, float scale, void* out_dev, int64_t out_ld, int32_t out_dtype) {
     return guard([&] {
-        AttnArgs A{};
-        A.L = bkv_layer(ctx, cache, layer);
-        A.S = bkv_streams(batch);
+        BkvAttn a{};
+        a.L = bkv_layer(ctx, cache, layer);
+        a.S = bkv_streams(batch);
         if (n_head <= 0 || n_head % cache->n_kv_head)
             fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: n_head must be a multiple of n_kv_head");
         for (int dt : {q_dtype, out_dtype})
             if (dt != VKB_DT_F32 && dt != VKB_DT_F16) fail(VKB_ERROR_UNSUPPORTED_OP, "bkv_attention: q and out must be F32 or F16");
-        const int64_t width = (int64_t)n_head * cache->d_head;
+        a.d_head = cache->d_head;
+        const int64_t width = (int64_t)n_head * a.d_head;
         if (q_ld < width || out_ld < width) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: row stride below n_head*d_head");
         if (!(scale > 0.0f) || scale > 3.0e38f) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: scale must be positive and finite");
         if (batch->n_seq == 0 || batch->n_tok == 0) return;
         if (!q_dev || !out_dev) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: null q/out");
-        A.group = n_head / cache->n_kv_head;
-        A.n_head = n_head;
-        if ((int64_t)batch->n_tok * A.group > INT32_MAX / 2) fail(VKB_ERROR_UNSUPPORTED_OP, "bkv_attention: too many rows");
-        A.q_f16 = q_dtype == VKB_DT_F16;
-        A.out_f16 = out_dtype == VKB_DT_F16;
-        if ((uintptr_t)q_dev % (A.q_f16 ? 2 : 4) || (uintptr_t)out_dev % (A.out_f16 ? 2 : 4))
+        a.group = n_head / cache->n_kv_head;
+        a.n_head = n_head;
+        a.max_q = std::max(1, std::min(batch->max_q, batch->n_tok));
+        if ((int64_t)batch->n_tok * a.group > INT32_MAX / 2) fail(VKB_ERROR_UNSUPPORTED_OP, "bkv_attention: too many rows");
+        a.q_f16 = q_dtype == VKB_DT_F16;
+        a.out_f16 = out_dtype == VKB_DT_F16;
+        if ((uintptr_t)q_dev % (a.q_f16 ? 2 : 4) || (uintptr_t)out_dev % (a.out_f16 ? 2 : 4))
             fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: misaligned q/out");
-        A.q = q_dev;
-        A.q_ld = q_ld;
-        A.q_vec = (uintptr_t)q_dev % (A.q_f16 ? 8 : 16) == 0 && q_ld % 4 == 0;
-        A.out_vec = (uintptr_t)out_dev % (A.out_f16 ? 4 : 8) == 0 && out_ld % 2 == 0;
-        A.scale = scale;
-        A.out = out_dev;
-        A.out_ld = out_ld;
+        a.q = q_dev;
+        a.q_ld = q_ld;
+        a.scale = scale;
+        a.out = out_dev;
+        a.out_ld = out_ld;
         NvtxRange nvtx_range("vkb.bkv.attention");
-        with_bkv_head(cache->d_head, [&](auto D) {
-            if (!A.q_f16 || !A.out_f16) launch_attn<decltype(D)::value, true, true>(ctx, A);
-            else if ((int64_t)batch->max_q * A.group <= 8) launch_attn<decltype(D)::value, true, false>(ctx, A);
-            else launch_attn<decltype(D)::value, false, false>(ctx, A);
-        });
+        if (bkv_prompt_takes(ctx, a)) run_bkv_prompt(ctx, a);
+        else run_bkv_attn(ctx, a);
     });
 }

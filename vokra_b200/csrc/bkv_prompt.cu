@@ -1,0 +1,461 @@
+// bkv_prompt.cu — attention over the block-scaled 8-bit KV cache for many query
+// rows a stream (prompts and chunks of them), 16-bit rows, on the fifth-generation
+// tensor cores.
+//
+// Bound: three things that come to about the same at d_head 128: the products
+// (2 x 2 x 256 x 128 x 128 operations a step at 8192 a cycle and SM: 2048 cycles),
+// the exponentials (256 x 128 at 16 a cycle: 2048) and the shared memory that
+// the products read. So a block keeps two tiles of 128 query rows (of one KV head:
+// row = token * group + head) that share each K/V tile of 128 keys, and while one
+// tile's softmax runs the other one's products do:
+//   warps 0..3, 4..7  softmax of tile 0, 1: thread = row = its own lane of tensor
+//                     memory, so a row's maximum and sum need no exchange
+//   warps 8..11       K and V pages from global memory, int8 -> f16 (exact), into
+//                     shared memory with the 128-byte swizzle; V pages are stored
+//                     channel by channel, which is the K-major operand of P.V, so
+//                     nothing is transposed. The next tile's pages are in
+//                     registers while this one is converted.
+//   warp 12           issues the products: S = Q K^T from shared memory, O += P V
+//                     with P (f16) in tensor memory, in S's own columns. It takes
+//                     whichever tile is ready.
+// Scales stay in fp32: a block's K scale multiplies its scores in the exponent's
+// own multiply-add; its V scale, over a running power of two `frame`, is added to
+// the exponent as a logarithm, so a weight comes out scaled at no cost, and the
+// row's sum takes the 16 weights of a block times the inverse. The running
+// maximum (and O) is raised only when a tile exceeds it by 2^8.
+#include "bkv_attn.cuh"
+#include "tc_ptx.cuh"
+
+namespace vkb {
+namespace {
+
+constexpr int ROWS = 256;           // query rows of a block, two tiles of 128
+constexpr int KEYS = 128;           // keys of a step
+constexpr int PAGES = KEYS / BKV_BLOCK;
+constexpr int THREADS = 13 * 32;
+constexpr uint32_t TMEM_COLS = 512;
+constexpr float L2E = 1.4426950408889634f;
+constexpr float RAISE = 8.0f;       // log2
+constexpr float MIN_W = 9.5367431640625e-7f;  // 2^-20: V scales further below the frame than this count as this
+constexpr uint32_t POLLS = 1u << 26;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct StepScales {
+    float k[PAGES];   // K scale * softmax scale * log2(e)
+    float lw[PAGES];  // log2 of the V scale over the frame; -inf: the page is not there
+    float iw[PAGES];  // the inverse of that V scale over the frame; 0 where the page is not there
+    float turn;       // the last step's frame over this one's
+    float frame;
+    int missing;      // whether a page is not there
+};
+
+template <int D>
+struct Smem {
+    static constexpr int TILE = KEYS * D * 2;  // a tile of Q, K or V as f16
+    static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, SC = 6 * TILE;
+    static constexpr int BARS = SC + 4 * (int)sizeof(StepScales);
+    static constexpr int BYTES = 1024 + (BARS + 7) / 8 * 8 + 20 * 8;
+};
+
+// Byte offset of the 16-byte chunk `chunk` of row `row` in a block of rows of 128 bytes, swizzled.
+__device__ __forceinline__ uint32_t sw128(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// 16 int8 as 16 f16, in order (two chunks).
+__device__ __forceinline__ void to_f16(const uint4& v, uint4& a, uint4& b) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t o[8];
+    const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));  // 1152
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = w[i] ^ 0x80808080u;
+        const uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&lo), bias);
+        const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&hi), bias);
+        o[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+        o[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    a = make_uint4(o[0], o[1], o[2], o[3]);
+    b = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* err) {
+    pdl_entry();
+    using M = Smem<D>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the block's row tile: number x of all streams' tiles, found by every warp for itself
+    const int h = (int)(blockIdx.x % A.L.n_kv_head);
+    int x = (int)(blockIdx.x / A.L.n_kv_head), s = -1, first_row = 0, n_q = 0, tile = 0;
+    for (int base = 0; base < A.S.n_seq && s < 0; base += 32) {
+        int first = 0, n = 0;
+        if (base + lane < A.S.n_seq) A.S.rows(base + lane, first, n);
+        const int mine = (int)(((int64_t)n * A.group + ROWS - 1) / ROWS);
+        int sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += y;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, sum > x);
+        if (behind) {
+            const int at = __ffs(behind) - 1;
+            s = base + at;
+            first_row = __shfl_sync(0xffffffffu, first, at);
+            n_q = __shfl_sync(0xffffffffu, n, at);
+            // a stream's last tile sees the most keys: it comes first
+            tile = __shfl_sync(0xffffffffu, sum, at) - 1 - x;
+        } else {
+            x -= __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+    if (s < 0) return;
+    const int n_rows = n_q * A.group, row0 = tile * ROWS;
+    const int n_keys = A.S.keys(s);
+    // keys that row r sees: those up to its token's position
+    auto limit_of = [&](int r) { return r < n_rows ? max(0, min(n_keys, n_keys - n_q + r / A.group + 1)) : 0; };
+    const int n_steps = (limit_of(min(n_rows, row0 + ROWS) - 1) + KEYS - 1) / KEYS;
+
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
+    StepScales* scales = reinterpret_cast<StepScales*>(smem + M::SC);  // [4]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (M::BARS + 7) / 8 * 8);
+    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7,
+             *s_full = bars + 9, *p_full = bars + 11, *pv_done = bars + 13;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+    if (threadIdx.x == 0) {
+        ptx::mbar_init(q_full, 256);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&k_full[i], 128);
+            ptx::mbar_init(&v_full[i], 128);
+            ptx::mbar_init(&k_empty[i], 1);
+            ptx::mbar_init(&v_empty[i], 1);
+            ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&p_full[i], 128);
+            ptx::mbar_init(&pv_done[i], 1);
+        }
+        ptx::fence_mbar_init();
+    }
+    if (warp == 12) {
+        ptx::tmem_alloc(tmem_slot, TMEM_COLS);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t S_COL = 0, O_COL = 256;  // S (and P) of tile t at 128 t, O at 256 + D t
+    bool ok = true;
+
+    if (warp < 8) {
+        // ---- softmax and epilogue: thread = row
+        const int t = warp >> 2, quarter = warp & 3;
+        const int r = row0 + t * 128 + quarter * 32 + lane;
+        const int tok = r / A.group, head = h * A.group + r % A.group;
+        const int limit = limit_of(r);
+        {
+            const __half* q = reinterpret_cast<const __half*>(A.q) + (int64_t)(first_row + tok) * A.q_ld + (int64_t)head * D;
+            uint8_t* to = smem + M::Q + t * M::TILE;
+            const int row = quarter * 32 + lane;
+            uint4 v[D / 8];
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+                v[i] = r < n_rows ? __ldcg(reinterpret_cast<const uint4*>(q) + i) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(to + (i >> 3) * (128 * 128) + sw128(row, i & 7)) = v[i];
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(q_full);
+        }
+        const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
+        const uint32_t s_at = at + S_COL + 128 * t, o_at = at + O_COL + D * t;
+        float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum
+        float frame = 1.0f;
+        for (int j = 0; j < n_steps && ok; ++j) {
+            if (!ptx::mbar_wait(&s_full[t], j & 1)) { ok = false; break; }
+            ptx::tc_fence_after();
+            const StepScales& sc = scales[j & 3];
+            const int left = limit - j * KEYS;  // the row sees the step's first `left` keys
+            const bool masked = __any_sync(0xffffffffu, left < KEYS) || sc.missing;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int c0 = 0; c0 < KEYS; c0 += 32) {
+                uint32_t v[32];
+                ptx::tmem_ld32(s_at + c0, v);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int b = 0; b < 32; b += 16) {
+                    float bm = -INFINITY;
+                    if (!masked) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(v[b + c]));
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c)
+                            if (c0 + b + c < left) bm = fmaxf(bm, __uint_as_float(v[b + c]));
+                        if (sc.iw[(c0 + b) >> 4] == 0.0f) bm = -INFINITY;
+                    }
+                    mx = fmaxf(mx, bm == -INFINITY ? bm : bm * sc.k[(c0 + b) >> 4]);
+                }
+            }
+            const bool raise = mx > m + RAISE;
+            const float m_new = raise ? mx : m;
+            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+            const float corr = (raise ? ex2(m - m_use) : 1.0f);
+            const float corr_o = corr * sc.turn;
+            // O is at rest: this step's scores came after the last P.V
+            if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
+#pragma unroll
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    ptx::tmem_ld32(o_at + c0, o);
+                    ptx::tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr_o);
+                    ptx::tmem_st32(o_at + c0, o);
+                }
+            }
+            l *= corr;
+            m = m_new;
+            frame = sc.frame;
+            // P over S, 32 columns of scores becoming 16 of f16 pairs: only columns that have been read are overwritten
+#pragma unroll
+            for (int c0 = 0; c0 < KEYS; c0 += 32) {
+                uint32_t v[32], p[16];
+                ptx::tmem_ld32(s_at + c0, v);
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int b = 0; b < 32; b += 16) {
+                    const float k = sc.k[(c0 + b) >> 4], add = sc.lw[(c0 + b) >> 4] - m_use;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int c = 0; c < 16; c += 2) {
+                        float x = ex2(fmaf(__uint_as_float(v[b + c]), k, add)), y = ex2(fmaf(__uint_as_float(v[b + c + 1]), k, add));
+                        if (masked) {
+                            if (c0 + b + c >= left) x = 0.0f;
+                            if (c0 + b + c + 1 >= left) y = 0.0f;
+                        }
+                        sum += x + y;
+                        const __half2 hp = __floats2half2_rn(x, y);
+                        p[(b + c) >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                    }
+                    l = fmaf(sum, sc.iw[(c0 + b) >> 4], l);
+                }
+                ptx::tmem_st16(s_at + (c0 >> 1), p);
+            }
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(&p_full[t]);
+        }
+        if (ok && n_steps > 0 && !ptx::mbar_wait(&pv_done[t], (n_steps - 1) & 1)) ok = false;
+        if (ok) {
+            ptx::tc_fence_after();
+            const float fin = frame / l;
+            __half* to = reinterpret_cast<__half*>(A.out) + (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D;
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 32) {
+                uint32_t o[32];
+                if (n_steps > 0) {
+                    ptx::tmem_ld32(o_at + c0, o);
+                    ptx::tmem_ld_wait();
+                }
+                if (r < n_rows) {
+                    __align__(16) __half2 y[16];
+#pragma unroll
+                    for (int c = 0; c < 16; ++c)
+                        y[c] = l == 0.0f ? __floats2half2_rn(0.0f, 0.0f)
+                                         : __floats2half2_rn(__uint_as_float(o[2 * c]) * fin, __uint_as_float(o[2 * c + 1]) * fin);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) reinterpret_cast<uint4*>(to + c0)[c] = reinterpret_cast<const uint4*>(y)[c];
+                }
+            }
+        }
+    } else if (warp < 12) {
+        // ---- K and V: thread = 16 bytes of page (i * PER + sub), i = 0 .. N - 1
+        constexpr int G = D / 16;              // 16-byte groups of a K row
+        constexpr int PER = 128 / (16 * G);    // pages that 128 threads take at a time (D = 128: 1, 64: 2)
+        constexpr int N = PAGES / PER;
+        const int tid = threadIdx.x - 256, sub = tid / (16 * G), in = tid % (16 * G);
+        const int n_pages = (n_keys + BKV_BLOCK - 1) / BKV_BLOCK;
+        auto ids_of = [&](int j) {  // lane i < 8: page i of step j
+            const int p = j * PAGES + lane;
+            return j < n_steps && lane < PAGES && p < n_pages ? (int)A.S.page(s, p, A.L.n_pages) : -1;
+        };
+        auto load = [&](const int8_t* arena, int ids, uint4 (&v)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int id = __shfl_sync(0xffffffffu, ids, i * PER + sub);
+                v[i] = id >= 0 ? __ldcg(reinterpret_cast<const uint4*>(arena + ((int64_t)id * A.L.n_kv_head + h) * (BKV_BLOCK * D)) + in)
+                               : make_uint4(0, 0, 0, 0);
+            }
+        };
+        int ids = ids_of(0), ids_next = ids_of(1);
+        uint4 kv[N], vv[N];
+        load(A.L.k, ids, kv);
+        float ks = 0.0f, vs = 0.0f;
+        auto load_scales = [&](int id) {
+            ks = id >= 0 ? __ldcg(A.L.ks + (int64_t)id * A.L.n_kv_head + h) : 0.0f;
+            vs = id >= 0 ? __ldcg(A.L.vs + (int64_t)id * A.L.n_kv_head + h) : 0.0f;
+        };
+        if (warp == 8) load_scales(ids);
+        load(A.L.v, ids, vv);
+        float frame = __uint_as_float(0x00800000u);
+        for (int j = 0; j < n_steps && ok; ++j) {
+            const int st = j & 1;
+            // K: token = row of the operand, channels in blocks of 64
+            if (!ptx::mbar_wait(&k_empty[st], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
+            {
+                uint8_t* to = smem + M::K + st * M::TILE;
+                const int tok = in / G, grp = in % G;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    uint4 a, b;
+                    to_f16(kv[i], a, b);
+                    const int row = (i * PER + sub) * BKV_BLOCK + tok, c = 2 * (grp & 3);
+                    uint8_t* blk = to + (grp >> 2) * (KEYS * 128);
+                    // the two 64-channel blocks take their chunks in opposite order: no two lanes meet in a bank
+                    const bool swap = grp >> 2;
+                    *reinterpret_cast<uint4*>(blk + sw128(row, c + swap)) = swap ? b : a;
+                    *reinterpret_cast<uint4*>(blk + sw128(row, c + !swap)) = swap ? a : b;
+                }
+            }
+            if (warp == 8) {
+                // (scales[j & 3] was last read for step j - 4, which ended before K's buffer of step j - 2 came free)
+                StepScales& sc = scales[j & 3];
+                float vmax = vs;
+#pragma unroll
+                for (int o = 4; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+                const float pow2 = fmaxf(frame, __uint_as_float(__float_as_uint(vmax) & 0x7f800000u));
+                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(pow2));
+                const unsigned there = __ballot_sync(0xffffffffu, ids >= 0);
+                if (lane < PAGES) {
+                    const float w = fmaxf(vs * inv, MIN_W);
+                    sc.k[lane] = ks * (A.scale * L2E);
+                    sc.lw[lane] = ids >= 0 ? log2f(w) : -INFINITY;
+                    sc.iw[lane] = ids >= 0 ? 1.0f / w : 0.0f;
+                }
+                const int valid = min(PAGES, n_pages - j * PAGES);
+                if (lane == 0) {
+                    sc.turn = j ? frame * inv : 1.0f;
+                    sc.frame = pow2;
+                    sc.missing = (there & ((1u << valid) - 1)) != (1u << valid) - 1;
+                }
+                frame = __shfl_sync(0xffffffffu, pow2, 0);
+                __syncwarp();
+            }
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(&k_full[st]);
+            const int ids_now = ids_next;
+            if (j + 1 < n_steps) {
+                load(A.L.k, ids_now, kv);
+                if (warp == 8) load_scales(ids_now);
+            }
+            ids_next = ids_of(j + 2);
+            // V: channel = row of the operand, keys in blocks of 64
+            if (!ptx::mbar_wait(&v_empty[st], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
+            {
+                uint8_t* to = smem + M::V + st * M::TILE;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    uint4 a, b;
+                    to_f16(vv[i], a, b);
+                    const int page = i * PER + sub;
+                    uint8_t* blk = to + (page >> 2) * (D * 128);
+                    *reinterpret_cast<uint4*>(blk + sw128(in, 2 * (page & 3))) = a;
+                    *reinterpret_cast<uint4*>(blk + sw128(in, 2 * (page & 3) + 1)) = b;
+                }
+            }
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(&v_full[st]);
+            if (j + 1 < n_steps) load(A.L.v, ids_now, vv);
+            ids = ids_now;
+        }
+    } else if (lane == 0 && n_steps > 0) {
+        // ---- the products. Tile t is at its S of step s_next[t], or at its P.V of step pv_next[t]
+        constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, KEYS), idesc_o = ptx::idesc_f16_f32(128, D);
+        const uint32_t q_addr = ptx::smem_u32(smem + M::Q), k_addr = ptx::smem_u32(smem + M::K), v_addr = ptx::smem_u32(smem + M::V);
+        int s_next[2] = {0, 0}, pv_next[2] = {0, 0};
+        ok = ptx::mbar_wait(q_full, 0);
+        uint32_t polls = 0;
+        while (ok && (pv_next[0] < n_steps || pv_next[1] < n_steps)) {
+            bool moved = false;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if (pv_next[t] < s_next[t]) {
+                    const int j = pv_next[t];
+                    if (ptx::mbar_test(&p_full[t], j & 1) && ptx::mbar_test(&v_full[j & 1], (j >> 1) & 1)) {
+                        ptx::tc_fence_after();
+                        const uint32_t b = v_addr + (j & 1) * M::TILE;
+#pragma unroll
+                        for (int kk = 0; kk < KEYS / 16; ++kk)
+                            ptx::mma_f16_ts(tmem + O_COL + D * t, tmem + S_COL + 128 * t + kk * 8,
+                                            ptx::sdesc_sw128(b + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o,
+                                            (j > 0 || kk > 0) ? 1u : 0u);
+                        ptx::mma_commit(&pv_done[t]);
+                        ++pv_next[t];
+                        if (pv_next[t ^ 1] > j) ptx::mma_commit(&v_empty[j & 1]);
+                        moved = true;
+                    }
+                } else if (s_next[t] < n_steps) {
+                    const int j = s_next[t];
+                    // S overwrites the columns of the last step's P: that P.V must be complete
+                    if (ptx::mbar_test(&k_full[j & 1], (j >> 1) & 1) && (j == 0 || ptx::mbar_test(&pv_done[t], (j - 1) & 1))) {
+                        ptx::tc_fence_after();
+                        const uint32_t a = q_addr + t * M::TILE, b = k_addr + (j & 1) * M::TILE;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            ptx::mma_f16_ss(tmem + S_COL + 128 * t, ptx::sdesc_sw128(a + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
+                                            ptx::sdesc_sw128(b + (kk >> 2) * (KEYS * 128) + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
+                        ptx::mma_commit(&s_full[t]);
+                        ++s_next[t];
+                        if (s_next[t ^ 1] > j) ptx::mma_commit(&k_empty[j & 1]);
+                        moved = true;
+                    }
+                }
+            }
+            if (moved) polls = 0;
+            else if (++polls == POLLS) ok = false;
+        }
+    }
+    if (!ok) atomicExch(err, 1);
+    __syncwarp();
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, TMEM_COLS);
+    }
+}
+
+int64_t most_tiles(const BkvAttn& a) { return (int64_t)a.S.n_tok * a.group / ROWS + a.S.n_seq; }
+
+template <int D>
+void launch(vkb_context* ctx, const BkvAttn& a) {
+    auto kern = bkv_prompt_kernel<D>;
+    static_assert(Smem<D>::BYTES <= 227 * 1024, "shared memory of one block");
+    smem_optin(kern, Smem<D>::BYTES);
+    // (at most) as many row tiles: the rows of all streams, and one begun tile for each
+    const int64_t blocks = most_tiles(a) * a.L.n_kv_head;
+    if (blocks > INT32_MAX) fail(VKB_ERROR_UNSUPPORTED_OP, "bkv_attention: too many rows");
+    launch_pdl(ctx, kern, dim3((unsigned)blocks), THREADS, Smem<D>::BYTES, a, ctx->err_flag.as<int>());
+    VKB_CUDA(cudaGetLastError());
+    ctx->count();
+}
+
+}  // namespace
+
+bool bkv_prompt_takes(const vkb_context* ctx, const BkvAttn& a) {
+    if (!a.q_f16 || !a.out_f16 || (a.d_head != 64 && a.d_head != 128)) return false;
+    if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_ld % 8 || a.out_ld % 8) return false;
+    return (int64_t)a.max_q * a.group >= 64 && (int64_t)a.S.n_tok * a.group / ROWS * a.L.n_kv_head >= 16;
+}
+
+void run_bkv_prompt(vkb_context* ctx, const BkvAttn& a) {
+    if (a.d_head == 64) launch<64>(ctx, a);
+    else launch<128>(ctx, a);
+}
+
+}  // namespace vkb
