@@ -125,8 +125,8 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
     StepScales* scales = reinterpret_cast<StepScales*>(smem + M::SC);  // [4]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (M::BARS + 7) / 8 * 8);
     uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7,
-             *s_full = bars + 9, *p_full = bars + 11, *pv_done = bars + 13;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+             *s_full = bars + 9, *p_half = bars + 11, *p_full = bars + 13, *pv_done = bars + 15;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
     if (threadIdx.x == 0) {
         ptx::mbar_init(q_full, 256);
         for (int i = 0; i < 2; ++i) {
@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             ptx::mbar_init(&k_empty[i], 1);
             ptx::mbar_init(&v_empty[i], 1);
             ptx::mbar_init(&s_full[i], 1);
+            ptx::mbar_init(&p_half[i], 128);
             ptx::mbar_init(&p_full[i], 128);
             ptx::mbar_init(&pv_done[i], 1);
         }
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         const int t = warp >> 2, quarter = warp & 3;
         const int r = row0 + t * 128 + quarter * 32 + lane;
         const int tok = r / A.group, head = h * A.group + r % A.group;
-        const int limit = limit_of(r);
+        const int limit = r < n_rows ? limit_of(r) : INT32_MAX;  // (a row that is not there masks nothing and is not written)
         {
             const __half* q = reinterpret_cast<const __half*>(A.q) + (int64_t)(first_row + tok) * A.q_ld + (int64_t)head * D;
             uint8_t* to = smem + M::Q + t * M::TILE;
@@ -181,24 +182,28 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             const int left = limit - j * KEYS;  // the row sees the step's first `left` keys
             const bool masked = __any_sync(0xffffffffu, left < KEYS) || sc.missing;
             float mx = -INFINITY;
+            uint32_t v[2][32];  // 32 columns in hand, the next 32 on their way
+            auto mask = [&](uint32_t (&x)[32], int c0) {
+#pragma unroll
+                for (int b = 0; b < 32; b += 16) {
+                    const int n = sc.iw[(c0 + b) >> 4] == 0.0f ? 0 : left - c0 - b;  // of the page's tokens the row sees the first n
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) x[b + c] = c < n ? x[b + c] : __float_as_uint(-INFINITY);
+                }
+            };
+            ptx::tmem_ld32(s_at, v[0]);
 #pragma unroll
             for (int c0 = 0; c0 < KEYS; c0 += 32) {
-                uint32_t v[32];
-                ptx::tmem_ld32(s_at + c0, v);
-                ptx::tmem_ld_wait();
+                uint32_t(&x)[32] = v[(c0 >> 5) & 1];
+                ptx::tmem_ld_wait_for(x);
+                ptx::tmem_ld32(s_at + (c0 + 32) % KEYS, v[((c0 >> 5) + 1) & 1]);  // at the end: the first ones again
+                if (masked) mask(x, c0);
 #pragma unroll
                 for (int b = 0; b < 32; b += 16) {
                     float bm = -INFINITY;
-                    if (!masked) {
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(v[b + c]));
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 16; ++c)
-                            if (c0 + b + c < left) bm = fmaxf(bm, __uint_as_float(v[b + c]));
-                        if (sc.iw[(c0 + b) >> 4] == 0.0f) bm = -INFINITY;
-                    }
-                    mx = fmaxf(mx, bm == -INFINITY ? bm : bm * sc.k[(c0 + b) >> 4]);
+                    for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(x[b + c]));
+                    mx = fmaxf(mx, bm * sc.k[(c0 + b) >> 4]);
                 }
             }
             const bool raise = mx > m + RAISE;
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     uint32_t o[32];
                     ptx::tmem_ld32(o_at + c0, o);
-                    ptx::tmem_ld_wait();
+                    ptx::tmem_ld_wait_for(o);
 #pragma unroll
                     for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr_o);
                     ptx::tmem_st32(o_at + c0, o);
@@ -221,34 +226,39 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             l *= corr;
             m = m_new;
             frame = sc.frame;
-            // P over S, 32 columns of scores becoming 16 of f16 pairs: only columns that have been read are overwritten
+            // P over S, 32 columns of scores becoming 16 of f16 pairs: only columns that have been read are overwritten.
+            // The first half of P goes to its product while the second one is made
 #pragma unroll
             for (int c0 = 0; c0 < KEYS; c0 += 32) {
-                uint32_t v[32], p[16];
-                ptx::tmem_ld32(s_at + c0, v);
-                ptx::tmem_ld_wait();
+                uint32_t(&w)[32] = v[(c0 >> 5) & 1];
+                ptx::tmem_ld_wait_for(w);
+                if (c0 + 32 < KEYS) ptx::tmem_ld32(s_at + c0 + 32, v[((c0 >> 5) + 1) & 1]);
+                if (masked) mask(w, c0);
+                uint32_t p[16];
 #pragma unroll
                 for (int b = 0; b < 32; b += 16) {
+                    const uint32_t* x = w + b;
                     const float k = sc.k[(c0 + b) >> 4], add = sc.lw[(c0 + b) >> 4] - m_use;
-                    float sum = 0.0f;
+                    const float2 k2 = make_float2(k, k), add2 = make_float2(add, add);
+                    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                     for (int c = 0; c < 16; c += 2) {
-                        float x = ex2(fmaf(__uint_as_float(v[b + c]), k, add)), y = ex2(fmaf(__uint_as_float(v[b + c + 1]), k, add));
-                        if (masked) {
-                            if (c0 + b + c >= left) x = 0.0f;
-                            if (c0 + b + c + 1 >= left) y = 0.0f;
-                        }
-                        sum += x + y;
-                        const __half2 hp = __floats2half2_rn(x, y);
+                        float2 y = __ffma2_rn(make_float2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), k2, add2);
+                        y.x = ex2(y.x);
+                        y.y = ex2(y.y);
+                        sum = __fadd2_rn(sum, y);
+                        const __half2 hp = __floats2half2_rn(y.x, y.y);
                         p[(b + c) >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
-                    l = fmaf(sum, sc.iw[(c0 + b) >> 4], l);
+                    l = fmaf(sum.x + sum.y, sc.iw[(c0 + b) >> 4], l);
                 }
                 ptx::tmem_st16(s_at + (c0 >> 1), p);
+                if (c0 + 32 == KEYS / 2 || c0 + 32 == KEYS) {
+                    ptx::tmem_st_wait();
+                    ptx::tc_fence_before();
+                    ptx::mbar_arrive(c0 + 32 == KEYS ? &p_full[t] : &p_half[t]);
+                }
             }
-            ptx::tmem_st_wait();
-            ptx::tc_fence_before();
-            ptx::mbar_arrive(&p_full[t]);
         }
         if (ok && n_steps > 0 && !ptx::mbar_wait(&pv_done[t], (n_steps - 1) & 1)) ok = false;
         if (ok) {
@@ -333,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 const unsigned there = __ballot_sync(0xffffffffu, ids >= 0);
                 if (lane < PAGES) {
                     const float w = fmaxf(vs * inv, MIN_W);
-                    sc.k[lane] = ks * (A.scale * L2E);
+                    sc.k[lane] = fmaxf(ks * (A.scale * L2E), 1e-37f);  // above 0: a masked -inf stays -inf
                     sc.lw[lane] = ids >= 0 ? log2f(w) : -INFINITY;
                     sc.iw[lane] = ids >= 0 ? 1.0f / w : 0.0f;
                 }
@@ -373,48 +383,54 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             if (j + 1 < n_steps) load(A.L.v, ids_now, vv);
             ids = ids_now;
         }
-    } else if (lane == 0 && n_steps > 0) {
-        // ---- the products. Tile t is at its S of step s_next[t], or at its P.V of step pv_next[t]
+    } else if (n_steps > 0) {
+        // ---- the products, by the whole warp in step. Tile t is at its step[t]: S, the first half of P.V, the second half
         constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, KEYS), idesc_o = ptx::idesc_f16_f32(128, D);
-        const uint32_t q_addr = ptx::smem_u32(smem + M::Q), k_addr = ptx::smem_u32(smem + M::K), v_addr = ptx::smem_u32(smem + M::V);
-        int s_next[2] = {0, 0}, pv_next[2] = {0, 0};
-        ok = ptx::mbar_wait(q_full, 0);
+        const uint64_t q_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::Q)), k_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::K)),
+                       v_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::V));  // + bytes / 16: another place
+        auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xffffffffu, ptx::mbar_test(bar, parity)) != 0; };
+        int step[2] = {0, 0}, stage[2] = {0, 0};
+        ok = __all_sync(0xffffffffu, ptx::mbar_wait(q_full, 0));
         uint32_t polls = 0;
-        while (ok && (pv_next[0] < n_steps || pv_next[1] < n_steps)) {
+        while (ok && (step[0] < n_steps || step[1] < n_steps)) {
             bool moved = false;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                if (pv_next[t] < s_next[t]) {
-                    const int j = pv_next[t];
-                    if (ptx::mbar_test(&p_full[t], j & 1) && ptx::mbar_test(&v_full[j & 1], (j >> 1) & 1)) {
-                        ptx::tc_fence_after();
-                        const uint32_t b = v_addr + (j & 1) * M::TILE;
-#pragma unroll
-                        for (int kk = 0; kk < KEYS / 16; ++kk)
-                            ptx::mma_f16_ts(tmem + O_COL + D * t, tmem + S_COL + 128 * t + kk * 8,
-                                            ptx::sdesc_sw128(b + (kk >> 2) * (D * 128) + (kk & 3) * 32), idesc_o,
-                                            (j > 0 || kk > 0) ? 1u : 0u);
-                        ptx::mma_commit(&pv_done[t]);
-                        ++pv_next[t];
-                        if (pv_next[t ^ 1] > j) ptx::mma_commit(&v_empty[j & 1]);
-                        moved = true;
-                    }
-                } else if (s_next[t] < n_steps) {
-                    const int j = s_next[t];
+                const int j = step[t], st = j & 1, round = (j >> 1) & 1;
+                if (j >= n_steps) continue;
+                if (stage[t] == 0) {
+                    // the second tile starts half a step behind the first one, so that one's exponentials meet the other's products
+                    if (t == 1 && j == 0 && step[0] == 0 && stage[0] < 2) continue;
                     // S overwrites the columns of the last step's P: that P.V must be complete
-                    if (ptx::mbar_test(&k_full[j & 1], (j >> 1) & 1) && (j == 0 || ptx::mbar_test(&pv_done[t], (j - 1) & 1))) {
-                        ptx::tc_fence_after();
-                        const uint32_t a = q_addr + t * M::TILE, b = k_addr + (j & 1) * M::TILE;
+                    if (!ready(&k_full[st], round) || (j > 0 && !ready(&pv_done[t], (j - 1) & 1))) continue;
+                    ptx::tc_fence_after();
+                    const uint64_t a = q_desc + t * (M::TILE / 16), b = k_desc + st * (M::TILE / 16);
 #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            ptx::mma_f16_ss(tmem + S_COL + 128 * t, ptx::sdesc_sw128(a + (kk >> 2) * (128 * 128) + (kk & 3) * 32),
-                                            ptx::sdesc_sw128(b + (kk >> 2) * (KEYS * 128) + (kk & 3) * 32), idesc_s, kk > 0 ? 1u : 0u);
-                        ptx::mma_commit(&s_full[t]);
-                        ++s_next[t];
-                        if (s_next[t ^ 1] > j) ptx::mma_commit(&k_empty[j & 1]);
-                        moved = true;
+                    for (int kk = 0; kk < D / 16; ++kk)
+                        ptx::mma_f16_ss_warp(tmem + S_COL + 128 * t, a + ((kk >> 2) * (128 * 128) + (kk & 3) * 32) / 16,
+                                             b + ((kk >> 2) * (KEYS * 128) + (kk & 3) * 32) / 16, idesc_s, kk > 0 ? 1u : 0u);
+                    ptx::mma_commit_warp(&s_full[t]);
+                    if (step[t ^ 1] > j || (stage[t ^ 1] > 0 && step[t ^ 1] == j)) ptx::mma_commit_warp(&k_empty[st]);
+                    stage[t] = 1;
+                } else {
+                    const int half = stage[t] - 1;
+                    if (!ready(half ? &p_full[t] : &p_half[t], j & 1) || !ready(&v_full[st], round)) continue;
+                    ptx::tc_fence_after();
+                    const uint64_t b = v_desc + (st * M::TILE + half * (D * 128)) / 16;
+#pragma unroll
+                    for (int kk = 0; kk < KEYS / 32; ++kk)
+                        ptx::mma_f16_ts_warp(tmem + O_COL + D * t, tmem + S_COL + 128 * t + half * 32 + kk * 8, b + kk * 32 / 16,
+                                             idesc_o, (j > 0 || half > 0 || kk > 0) ? 1u : 0u);
+                    if (half) {
+                        ptx::mma_commit_warp(&pv_done[t]);
+                        if (step[t ^ 1] > j) ptx::mma_commit_warp(&v_empty[st]);
+                        ++step[t];
+                        stage[t] = 0;
+                    } else {
+                        stage[t] = 2;
                     }
                 }
+                moved = true;
             }
             if (moved) polls = 0;
             else if (++polls == POLLS) ok = false;
