@@ -10,12 +10,12 @@
 // tile's softmax runs the other one's products do:
 //   warps 0..3, 4..7  softmax of tile 0, 1: thread = row = its own lane of tensor
 //                     memory, so a row's maximum and sum need no exchange
-//   warps 8..11       K and V pages from global memory, int8 -> f16 (exact), into
+//   warps 8..11, 12..14  K, V pages from global memory, int8 -> f16 (exact), into
 //                     shared memory with the 128-byte swizzle; V pages are stored
 //                     channel by channel, which is the K-major operand of P.V, so
 //                     nothing is transposed. The next tile's pages are in
 //                     registers while this one is converted.
-//   warp 12           issues the products: S = Q K^T from shared memory, O += P V
+//   warp 15           issues the products: S = Q K^T from shared memory, O += P V
 //                     with P (f16) in tensor memory, in S's own columns. It takes
 //                     whichever tile is ready.
 // Scales stay in fp32: a block's K scale multiplies its scores in the exponent's
@@ -32,12 +32,12 @@ namespace {
 constexpr int ROWS = 256;           // query rows of a block, two tiles of 128
 constexpr int KEYS = 128;           // keys of a step
 constexpr int PAGES = KEYS / BKV_BLOCK;
-constexpr int THREADS = 13 * 32;
+constexpr int THREADS = 16 * 32;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float L2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2
 constexpr float MIN_W = 9.5367431640625e-7f;  // 2^-20: V scales further below the frame than this count as this
-constexpr uint32_t POLLS = 1u << 26;
+constexpr uint32_t POLLS = 1u << 24;
 
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -59,7 +59,7 @@ struct Smem {
     static constexpr int TILE = KEYS * D * 2;  // a tile of Q, K or V as f16
     static constexpr int Q = 0, K = 2 * TILE, V = 4 * TILE, SC = 6 * TILE;
     static constexpr int BARS = SC + 4 * (int)sizeof(StepScales);
-    static constexpr int BYTES = 1024 + (BARS + 7) / 8 * 8 + 20 * 8;
+    static constexpr int BYTES = 1024 + (BARS + 7) / 8 * 8 + 24 * 8;
 };
 
 // Byte offset of the 16-byte chunk `chunk` of row `row` in a block of rows of 128 bytes, swizzled.
@@ -118,30 +118,31 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
     const int n_keys = A.S.keys(s);
     // keys that row r sees: those up to its token's position
     auto limit_of = [&](int r) { return r < n_rows ? max(0, min(n_keys, n_keys - n_q + r / A.group + 1)) : 0; };
-    const int n_steps = (limit_of(min(n_rows, row0 + ROWS) - 1) + KEYS - 1) / KEYS;
+    const int n_half = (limit_of(min(n_rows, row0 + ROWS) - 1) + KEYS / 2 - 1) / (KEYS / 2), n_steps = (n_half + 1) / 2;
 
     extern __shared__ uint8_t raw_smem[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~uintptr_t(1023));
     StepScales* scales = reinterpret_cast<StepScales*>(smem + M::SC);  // [4]
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (M::BARS + 7) / 8 * 8);
-    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7,
-             *s_full = bars + 9, *p_half = bars + 11, *p_full = bars + 13, *pv_done = bars + 15;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
+    uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7;
+    uint64_t *s_full = bars + 9, *p_full = bars + 13, *pv_done = bars + 17;  // [tile * 2 + half]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
     if (threadIdx.x == 0) {
         ptx::mbar_init(q_full, 256);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&k_full[i], 128);
-            ptx::mbar_init(&v_full[i], 128);
+            ptx::mbar_init(&v_full[i], 96);
             ptx::mbar_init(&k_empty[i], 1);
             ptx::mbar_init(&v_empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
             ptx::mbar_init(&s_full[i], 1);
-            ptx::mbar_init(&p_half[i], 128);
             ptx::mbar_init(&p_full[i], 128);
             ptx::mbar_init(&pv_done[i], 1);
         }
         ptx::fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 15) {
         ptx::tmem_alloc(tmem_slot, TMEM_COLS);
         ptx::tmem_relinquish();
     }
@@ -175,70 +176,64 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         const uint32_t s_at = at + S_COL + 128 * t, o_at = at + O_COL + D * t;
         float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum
         float frame = 1.0f;
-        for (int j = 0; j < n_steps && ok; ++j) {
-            if (!ptx::mbar_wait(&s_full[t], j & 1)) { ok = false; break; }
+        for (int i = 0; i < n_half && ok; ++i) {
+            const int j = i >> 1, half = i & 1;
+            if (!ptx::mbar_wait(&s_full[2 * t + half], j & 1)) { ok = false; break; }
             ptx::tc_fence_after();
             const StepScales& sc = scales[j & 3];
-            const int left = limit - j * KEYS;  // the row sees the step's first `left` keys
-            const bool masked = __any_sync(0xffffffffu, left < KEYS) || sc.missing;
+            const int left = limit - i * (KEYS / 2);  // the row sees the half's first `left` keys
+            const bool masked = __any_sync(0xffffffffu, left < KEYS / 2) || sc.missing;
+            uint32_t v[2][32];  // the row's scores
+            ptx::tmem_ld32(s_at + 64 * half, v[0]);
+            ptx::tmem_ld32(s_at + 64 * half + 32, v[1]);
+            ptx::tmem_ld_wait_for(v[0]);
+            ptx::tmem_ld_wait_for(v[1]);
             float mx = -INFINITY;
-            uint32_t v[2][32];  // 32 columns in hand, the next 32 on their way
-            auto mask = [&](uint32_t (&x)[32], int c0) {
 #pragma unroll
-                for (int b = 0; b < 32; b += 16) {
-                    const int n = sc.iw[(c0 + b) >> 4] == 0.0f ? 0 : left - c0 - b;  // of the page's tokens the row sees the first n
+            for (int b = 0; b < PAGES / 2; ++b) {
+                uint32_t* x = v[b >> 1] + 16 * (b & 1);
+                const int page = half * (PAGES / 2) + b;
+                if (masked) {
+                    const int n = sc.iw[page] == 0.0f ? 0 : left - 16 * b;  // of the page's tokens the row sees the first n
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) x[b + c] = c < n ? x[b + c] : __float_as_uint(-INFINITY);
+                    for (int c = 0; c < 16; ++c) x[c] = c < n ? x[c] : __float_as_uint(-INFINITY);
                 }
-            };
-            ptx::tmem_ld32(s_at, v[0]);
+                float bm = -INFINITY;
 #pragma unroll
-            for (int c0 = 0; c0 < KEYS; c0 += 32) {
-                uint32_t(&x)[32] = v[(c0 >> 5) & 1];
-                ptx::tmem_ld_wait_for(x);
-                ptx::tmem_ld32(s_at + (c0 + 32) % KEYS, v[((c0 >> 5) + 1) & 1]);  // at the end: the first ones again
-                if (masked) mask(x, c0);
-#pragma unroll
-                for (int b = 0; b < 32; b += 16) {
-                    float bm = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(x[b + c]));
-                    mx = fmaxf(mx, bm * sc.k[(c0 + b) >> 4]);
-                }
+                for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(x[c]));
+                mx = fmaxf(mx, bm * sc.k[page]);
             }
             const bool raise = mx > m + RAISE;
             const float m_new = raise ? mx : m;
             const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-            const float corr = (raise ? ex2(m - m_use) : 1.0f);
-            const float corr_o = corr * sc.turn;
-            // O is at rest: this step's scores came after the last P.V
-            if (j > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
+            const float corr = raise ? ex2(m - m_use) : 1.0f;
+            const float corr_o = half ? corr : corr * sc.turn;
+            if (i > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
+                // O has to be at rest: the last half's P.V is complete
+                if (!ptx::mbar_wait(&pv_done[2 * t + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }
+                ptx::tc_fence_after();
 #pragma unroll
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    uint32_t o[32];
-                    ptx::tmem_ld32(o_at + c0, o);
+                for (int c0 = 0; c0 < D; c0 += 16) {
+                    uint32_t o[16];
+                    ptx::tmem_ld16(o_at + c0, o);
                     ptx::tmem_ld_wait_for(o);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr_o);
-                    ptx::tmem_st32(o_at + c0, o);
+                    for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr_o);
+                    ptx::tmem_st16(o_at + c0, o);
                 }
             }
             l *= corr;
             m = m_new;
             frame = sc.frame;
-            // P over S, 32 columns of scores becoming 16 of f16 pairs: only columns that have been read are overwritten.
-            // The first half of P goes to its product while the second one is made
+            // P over S, 64 columns of scores (all in registers by now) becoming 32 of f16 pairs
 #pragma unroll
-            for (int c0 = 0; c0 < KEYS; c0 += 32) {
-                uint32_t(&w)[32] = v[(c0 >> 5) & 1];
-                ptx::tmem_ld_wait_for(w);
-                if (c0 + 32 < KEYS) ptx::tmem_ld32(s_at + c0 + 32, v[((c0 >> 5) + 1) & 1]);
-                if (masked) mask(w, c0);
+            for (int c0 = 0; c0 < 2; ++c0) {
                 uint32_t p[16];
 #pragma unroll
-                for (int b = 0; b < 32; b += 16) {
-                    const uint32_t* x = w + b;
-                    const float k = sc.k[(c0 + b) >> 4], add = sc.lw[(c0 + b) >> 4] - m_use;
+                for (int b = 0; b < 2; ++b) {
+                    const uint32_t* x = v[c0] + 16 * b;
+                    const int page = half * (PAGES / 2) + 2 * c0 + b;
+                    const float k = sc.k[page], add = sc.lw[page] - m_use;
                     const float2 k2 = make_float2(k, k), add2 = make_float2(add, add);
                     float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -248,19 +243,17 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                         y.y = ex2(y.y);
                         sum = __fadd2_rn(sum, y);
                         const __half2 hp = __floats2half2_rn(y.x, y.y);
-                        p[(b + c) >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                        p[8 * b + (c >> 1)] = *reinterpret_cast<const uint32_t*>(&hp);
                     }
-                    l = fmaf(sum.x + sum.y, sc.iw[(c0 + b) >> 4], l);
+                    l = fmaf(sum.x + sum.y, sc.iw[page], l);
                 }
-                ptx::tmem_st16(s_at + (c0 >> 1), p);
-                if (c0 + 32 == KEYS / 2 || c0 + 32 == KEYS) {
-                    ptx::tmem_st_wait();
-                    ptx::tc_fence_before();
-                    ptx::mbar_arrive(c0 + 32 == KEYS ? &p_full[t] : &p_half[t]);
-                }
+                ptx::tmem_st16(s_at + 64 * half + 16 * c0, p);
             }
+            ptx::tmem_st_wait();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(&p_full[2 * t + half]);
         }
-        if (ok && n_steps > 0 && !ptx::mbar_wait(&pv_done[t], (n_steps - 1) & 1)) ok = false;
+        if (ok && n_half > 0 && !ptx::mbar_wait(&pv_done[2 * t + ((n_half - 1) & 1)], ((n_half - 1) >> 1) & 1)) ok = false;
         if (ok) {
             ptx::tc_fence_after();
             const float fin = frame / l;
@@ -283,53 +276,73 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 }
             }
         }
-    } else if (warp < 12) {
-        // ---- K and V: thread = 16 bytes of page (i * PER + sub), i = 0 .. N - 1
-        constexpr int G = D / 16;              // 16-byte groups of a K row
-        constexpr int PER = 128 / (16 * G);    // pages that 128 threads take at a time (D = 128: 1, 64: 2)
-        constexpr int N = PAGES / PER;
-        const int tid = threadIdx.x - 256, sub = tid / (16 * G), in = tid % (16 * G);
+    } else if (warp < 15) {
+        // ---- warps 8..11: K, 12..14: V, in pieces of 16 bytes; the next step's are in registers while this one's are
+        // converted
+        const bool is_v = warp >= 12;
+        const int tid = threadIdx.x - (is_v ? 384 : 256);
+        constexpr int PIECES = PAGES * D;                   // of K or V of a step
+        constexpr int NK = PIECES / 128, NV = (PIECES + 95) / 96;
         const int n_pages = (n_keys + BKV_BLOCK - 1) / BKV_BLOCK;
+        const int8_t* arena = (is_v ? A.L.v : A.L.k) + (int64_t)h * (BKV_BLOCK * D);
+        const int64_t page_bytes = (int64_t)A.L.n_kv_head * (BKV_BLOCK * D);
         auto ids_of = [&](int j) {  // lane i < 8: page i of step j
             const int p = j * PAGES + lane;
             return j < n_steps && lane < PAGES && p < n_pages ? (int)A.S.page(s, p, A.L.n_pages) : -1;
         };
-        auto load = [&](const int8_t* arena, int ids, uint4 (&v)[N]) {
+        // K: two neighbouring tokens' four pieces of one 64-channel block lie in eight neighbouring lanes, whose chunks of the
+        // swizzled operand are in eight different banks; the lane bits are piece (2), token (1), block (D = 128), token (3)
+        constexpr int BLK = D / 64;
+        const int k_tok = ((tid >> 2) & 1) | (tid / (8 * BLK) & 7) << 1, k_blk = tid >> 3 & (BLK - 1), k_grp = 4 * k_blk + (tid & 3);
+        const int8_t* mine = arena + (is_v ? 0 : k_tok * D + 16 * k_grp);
+        uint4 raw[NV];
+        auto load = [&](int ids) {  // (a page that is not there reads page 0: its scores are masked)
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int id = __shfl_sync(0xffffffffu, ids, i * PER + sub);
-                v[i] = id >= 0 ? __ldcg(reinterpret_cast<const uint4*>(arena + ((int64_t)id * A.L.n_kv_head + h) * (BKV_BLOCK * D)) + in)
-                               : make_uint4(0, 0, 0, 0);
+            for (int i = 0; i < NV; ++i) {
+                const int piece = min(tid + (is_v ? 96 : 128) * i, PIECES - 1);
+                const int id = max(__shfl_sync(0xffffffffu, ids, piece / D), 0);
+                if (is_v || i < NK)
+                    raw[i] = __ldcg(reinterpret_cast<const uint4*>(mine + id * page_bytes + (is_v ? 16 * (piece % D) : 0)));
             }
         };
-        int ids = ids_of(0), ids_next = ids_of(1);
-        uint4 kv[N], vv[N];
-        load(A.L.k, ids, kv);
         float ks = 0.0f, vs = 0.0f;
         auto load_scales = [&](int id) {
             ks = id >= 0 ? __ldcg(A.L.ks + (int64_t)id * A.L.n_kv_head + h) : 0.0f;
             vs = id >= 0 ? __ldcg(A.L.vs + (int64_t)id * A.L.n_kv_head + h) : 0.0f;
         };
+        int ids = ids_of(0), ids_next = ids_of(1);
+        load(ids);
         if (warp == 8) load_scales(ids);
-        load(A.L.v, ids, vv);
         float frame = __uint_as_float(0x00800000u);
+        uint64_t *empty = is_v ? v_empty : k_empty, *full = is_v ? v_full : k_full;
         for (int j = 0; j < n_steps && ok; ++j) {
             const int st = j & 1;
-            // K: token = row of the operand, channels in blocks of 64
-            if (!ptx::mbar_wait(&k_empty[st], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
-            {
-                uint8_t* to = smem + M::K + st * M::TILE;
-                const int tok = in / G, grp = in % G;
+            if (!ptx::mbar_wait(&empty[st], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
+            if (!is_v) {
+                // token = row of the operand, channels in blocks of 64
+                const int row = 16 * (tid / D) + k_tok;
+                uint8_t* to = smem + M::K + st * M::TILE + k_blk * (KEYS * 128);
+                uint8_t* to_a = to + sw128(row, 2 * (tid & 3));
+                uint8_t* to_b = to + sw128(row, 2 * (tid & 3) + 1);
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
+                for (int i = 0; i < NK; ++i) {
                     uint4 a, b;
-                    to_f16(kv[i], a, b);
-                    const int row = (i * PER + sub) * BKV_BLOCK + tok, c = 2 * (grp & 3);
-                    uint8_t* blk = to + (grp >> 2) * (KEYS * 128);
-                    // the two 64-channel blocks take their chunks in opposite order: no two lanes meet in a bank
-                    const bool swap = grp >> 2;
-                    *reinterpret_cast<uint4*>(blk + sw128(row, c + swap)) = swap ? b : a;
-                    *reinterpret_cast<uint4*>(blk + sw128(row, c + !swap)) = swap ? a : b;
+                    to_f16(raw[i], a, b);
+                    *reinterpret_cast<uint4*>(to_a + i * (16 * (128 / D) * 128)) = a;  // whole pages on: the swizzle is the same
+                    *reinterpret_cast<uint4*>(to_b + i * (16 * (128 / D) * 128)) = b;
+                }
+            } else {
+                // channel = row of the operand, keys in blocks of 64
+                uint8_t* to = smem + M::V + st * M::TILE;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int piece = tid + 96 * i, page = piece / D, ch = piece % D;
+                    if (piece >= PIECES) break;
+                    uint4 a, b;
+                    to_f16(raw[i], a, b);
+                    uint8_t* blk = to + (page >> 2) * (D * 128);
+                    *reinterpret_cast<uint4*>(blk + sw128(ch, 2 * (page & 3))) = a;
+                    *reinterpret_cast<uint4*>(blk + sw128(ch, 2 * (page & 3) + 1)) = b;
                 }
             }
             if (warp == 8) {
@@ -357,90 +370,74 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 __syncwarp();
             }
             ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&k_full[st]);
-            const int ids_now = ids_next;
+            ptx::mbar_arrive(&full[st]);
+            ids = ids_next;
             if (j + 1 < n_steps) {
-                load(A.L.k, ids_now, kv);
-                if (warp == 8) load_scales(ids_now);
+                load(ids);
+                if (warp == 8) load_scales(ids);
             }
             ids_next = ids_of(j + 2);
-            // V: channel = row of the operand, keys in blocks of 64
-            if (!ptx::mbar_wait(&v_empty[st], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
-            {
-                uint8_t* to = smem + M::V + st * M::TILE;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    uint4 a, b;
-                    to_f16(vv[i], a, b);
-                    const int page = i * PER + sub;
-                    uint8_t* blk = to + (page >> 2) * (D * 128);
-                    *reinterpret_cast<uint4*>(blk + sw128(in, 2 * (page & 3))) = a;
-                    *reinterpret_cast<uint4*>(blk + sw128(in, 2 * (page & 3) + 1)) = b;
-                }
-            }
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(&v_full[st]);
-            if (j + 1 < n_steps) load(A.L.v, ids_now, vv);
-            ids = ids_now;
         }
     } else if (n_steps > 0) {
-        // ---- the products, by the whole warp in step. Tile t is at its step[t]: S, the first half of P.V, the second half
-        constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, KEYS), idesc_o = ptx::idesc_f16_f32(128, D);
+        // ---- the products, by the whole warp in step. Half i of a tile's keys has its scores in half i % 2 of the tile's
+        // columns, so S of the next half is made while this one's softmax runs. Tile t is at S of half s_at[t] and P.V of
+        // half pv_at[t]
+        constexpr uint32_t idesc_s = ptx::idesc_f16_f32(128, KEYS / 2), idesc_o = ptx::idesc_f16_f32(128, D);
         const uint64_t q_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::Q)), k_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::K)),
                        v_desc = ptx::sdesc_sw128(ptx::smem_u32(smem + M::V));  // + bytes / 16: another place
         auto ready = [&](uint64_t* bar, uint32_t parity) { return __any_sync(0xffffffffu, ptx::mbar_test(bar, parity)) != 0; };
-        int step[2] = {0, 0}, stage[2] = {0, 0};
+        int s_at[2] = {0, 0}, pv_at[2] = {0, 0};
         ok = __all_sync(0xffffffffu, ptx::mbar_wait(q_full, 0));
         uint32_t polls = 0;
-        while (ok && (step[0] < n_steps || step[1] < n_steps)) {
+        while (ok && (pv_at[0] < n_half || pv_at[1] < n_half)) {
             bool moved = false;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int j = step[t], st = j & 1, round = (j >> 1) & 1;
-                if (j >= n_steps) continue;
-                if (stage[t] == 0) {
-                    // the second tile starts half a step behind the first one, so that one's exponentials meet the other's products
-                    if (t == 1 && j == 0 && step[0] == 0 && stage[0] < 2) continue;
-                    // S overwrites the columns of the last step's P: that P.V must be complete
-                    if (!ready(&k_full[st], round) || (j > 0 && !ready(&pv_done[t], (j - 1) & 1))) continue;
-                    ptx::tc_fence_after();
-                    const uint64_t a = q_desc + t * (M::TILE / 16), b = k_desc + st * (M::TILE / 16);
+                if (pv_at[t] < s_at[t]) {
+                    const int i = pv_at[t], half = i & 1, st = (i >> 1) & 1;
+                    if (ready(&p_full[2 * t + half], (i >> 1) & 1) && ready(&v_full[st], (i >> 2) & 1)) {
+                        ptx::tc_fence_after();
+                        const uint64_t b = v_desc + (st * M::TILE + half * (D * 128)) / 16;
 #pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk)
-                        ptx::mma_f16_ss_warp(tmem + S_COL + 128 * t, a + ((kk >> 2) * (128 * 128) + (kk & 3) * 32) / 16,
-                                             b + ((kk >> 2) * (KEYS * 128) + (kk & 3) * 32) / 16, idesc_s, kk > 0 ? 1u : 0u);
-                    ptx::mma_commit_warp(&s_full[t]);
-                    if (step[t ^ 1] > j || (stage[t ^ 1] > 0 && step[t ^ 1] == j)) ptx::mma_commit_warp(&k_empty[st]);
-                    stage[t] = 1;
-                } else {
-                    const int half = stage[t] - 1;
-                    if (!ready(half ? &p_full[t] : &p_half[t], j & 1) || !ready(&v_full[st], round)) continue;
-                    ptx::tc_fence_after();
-                    const uint64_t b = v_desc + (st * M::TILE + half * (D * 128)) / 16;
-#pragma unroll
-                    for (int kk = 0; kk < KEYS / 32; ++kk)
-                        ptx::mma_f16_ts_warp(tmem + O_COL + D * t, tmem + S_COL + 128 * t + half * 32 + kk * 8, b + kk * 32 / 16,
-                                             idesc_o, (j > 0 || half > 0 || kk > 0) ? 1u : 0u);
-                    if (half) {
-                        ptx::mma_commit_warp(&pv_done[t]);
-                        if (step[t ^ 1] > j) ptx::mma_commit_warp(&v_empty[st]);
-                        ++step[t];
-                        stage[t] = 0;
-                    } else {
-                        stage[t] = 2;
+                        for (int kk = 0; kk < KEYS / 32; ++kk)
+                            ptx::mma_f16_ts_warp(tmem + O_COL + D * t, tmem + S_COL + 128 * t + 64 * half + kk * 8, b + kk * 32 / 16,
+                                                 idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+                        ptx::mma_commit_warp(&pv_done[2 * t + half]);
+                        ++pv_at[t];
+                        if (half && pv_at[t ^ 1] > i) ptx::mma_commit_warp(&v_empty[st]);
+                        moved = true;
                     }
                 }
-                moved = true;
+                if (s_at[t] < n_half) {
+                    const int i = s_at[t], half = i & 1, st = (i >> 1) & 1;
+                    // the columns held P of half i - 2: that P.V must be complete
+                    if (ready(&k_full[st], (i >> 2) & 1) && (i < 2 || (pv_at[t] > i - 2 && ready(&pv_done[2 * t + half], ((i >> 1) - 1) & 1)))) {
+                        ptx::tc_fence_after();
+                        const uint64_t a = q_desc + t * (M::TILE / 16), b = k_desc + (st * M::TILE + half * (KEYS / 2 * 128)) / 16;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; ++kk)
+                            ptx::mma_f16_ss_warp(tmem + S_COL + 128 * t + 64 * half, a + ((kk >> 2) * (128 * 128) + (kk & 3) * 32) / 16,
+                                                 b + ((kk >> 2) * (KEYS * 128) + (kk & 3) * 32) / 16, idesc_s, kk > 0 ? 1u : 0u);
+                        ptx::mma_commit_warp(&s_full[2 * t + half]);
+                        ++s_at[t];
+                        if (half && s_at[t ^ 1] > i) ptx::mma_commit_warp(&k_empty[st]);
+                        moved = true;
+                    }
+                }
             }
-            if (moved) polls = 0;
-            else if (++polls == POLLS) ok = false;
+            if (moved) {
+                polls = 0;
+            } else {
+                __nanosleep(20);
+                if (++polls == POLLS) ok = false;
+            }
         }
     }
     if (!ok) atomicExch(err, 1);
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 15) {
         ptx::tc_fence_after();
         ptx::tmem_dealloc(tmem, TMEM_COLS);
     }

@@ -248,6 +248,13 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
                    "+r"(r[30]), "+r"(r[31])::"memory");
 }
 
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15])::"memory");
+}
+
 // Shared-memory matrix descriptor (sm100 format): K-major operand whose rows
 // are 128 bytes wide with the 128-byte swizzle, 8-row core groups 1024 bytes
 // apart (SBO), start address in 16-byte units, descriptor version 1.
