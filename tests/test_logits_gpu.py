@@ -205,6 +205,22 @@ def test_rows_with_nothing_left_infinities_and_nan(ctx):
     assert abs(float(lp[7, 0])) <= LOGPROB_TOL and abs(float(lp[1, 0])) <= LOGPROB_TOL
 
 
+@pytest.mark.parametrize("left", [1, 31, 100, 700, 5000])
+@pytest.mark.parametrize("k", [1, 8, 32, 40, 64])
+def test_masks_that_leave_a_stretch_of_the_vocabulary(ctx, left, k):
+    """All candidates in a few neighbouring threads, in one window or over the border of two."""
+    from vokra_b200 import logits
+    rng = np.random.default_rng(left + k)
+    vocab, rows = 20000, 4
+    bits = np.zeros((rows, (vocab + 31) // 32 * 32), np.uint8)
+    for r, first in enumerate([0, 4000, 12288, vocab - left]):
+        bits[r, first:first + left] = 1
+    mask = np.packbits(bits, axis=1, bitorder="little").view(np.int32)
+    kw = {"mask": mask, "mask_row": np.arange(rows, dtype=np.int32)}
+    for x in ((rng.standard_normal((rows, vocab)) * 3).astype(np.float32), np.zeros((rows, vocab), np.float16)):
+        check_topk(plain_rules(x, vocab, **kw), k, *logits.topk(ctx, dev(x), k, rules_of(kw)))
+
+
 def test_all_rows_masked_and_no_rows(ctx):
     import torch
     from vokra_b200 import logits

@@ -25,9 +25,20 @@ namespace vkb {
 namespace {
 
 constexpr int LG_THREADS = 256;
+constexpr int WARPS = LG_THREADS / 32;
+constexpr float L2E = 1.4426950408889634f;
+constexpr uint32_t BANNED = 0x80000000u;  // in a count: the token completes an n-gram
+constexpr int HASH_BITS = 12, HASH = 1 << HASH_BITS;  // slots of the second pass's table of a row's history
 constexpr int TOPK_MAX = VKB_LOGITS_TOPK_MAX;
 constexpr int CAND = 512;                 // candidate buffer of the selection
-constexpr uint32_t BANNED = 0x80000000u;  // in a count: the token completes an n-gram
+constexpr int PRUNE_AT = 144;             // candidates that are worth a pass over them
+
+// 2^x on the special-function unit (relative error about 2^-22, -inf -> 0).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 struct Rules {
     const int32_t* hist;
@@ -70,6 +81,20 @@ struct RowRules {
     }
 };
 
+// The penalties of a token that occurs c times.
+__device__ __forceinline__ float penalized(const RowRules& rr, float x, uint32_t c) {
+    x = x > 0.0f ? __fdiv_rn(x, rr.rep) : __fmul_rn(x, rr.rep);
+    return __fsub_rn(x, __fadd_rn(__fmul_rn(rr.freq, (float)c), rr.pres));
+}
+
+// Whether id i of the history ends an n-gram whose first ngram - 1 ids are the history's last ones.
+__device__ __forceinline__ bool ends_ngram(const RowRules& rr, int ngram, int i) {
+    if (ngram <= 1 || i < ngram - 1) return false;
+    for (int e = 1; e < ngram; ++e)
+        if (rr.hist[i - e] != rr.hist[rr.n_hist - e]) return false;
+    return true;
+}
+
 template <typename T> struct Vec;
 template <> struct Vec<float> {
     static constexpr int N = 4;
@@ -85,110 +110,155 @@ template <> struct Vec<__half> {
 __device__ __forceinline__ void store1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void store1(__half* p, float x) { *p = __float2half_rn(x); }
 
+// How often each token of a window occurs in the row's history, in shared memory (integer adds: the order does not
+// matter), and a bit for each token that does, so that a look at the others costs a byte for eight.
+template <int TOKENS>
+struct History {
+    static constexpr int BYTES = (TOKENS + TOKENS / 32) * 4;
+    uint32_t *cnt, *bits;
+    // Counts for the window at `lo`; ends with a barrier.
+    __device__ __forceinline__ void count(const RowRules& rr, int ngram, uint32_t* smem, int lo, int vocab) {
+        cnt = smem;
+        bits = smem + TOKENS;
+        int id[4];
+        auto fetch = [&](int base) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = base + k * LG_THREADS + (int)threadIdx.x;
+                id[k] = i < rr.n_hist ? rr.hist[i] : -1;
+            }
+        };
+        fetch(0);
+        for (int i = threadIdx.x; i < BYTES / 16; i += LG_THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (int base = 0; base < rr.n_hist; base += 4 * LG_THREADS) {
+            if (base) fetch(base);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = id[k] - lo;
+                const bool here = id[k] >= 0 && id[k] < vocab && t >= 0 && t < TOKENS;
+                const unsigned with = __ballot_sync(0xffffffffu, here);
+                if (!here) continue;
+                int times = 1;
+                if (__popc(with) >= 8) {  // a loop of a few tokens would queue up at a few addresses: one lane adds for all equal ones
+                    const unsigned same = __match_any_sync(with, t);
+                    times = (int)(threadIdx.x & 31) == __ffs(same) - 1 ? __popc(same) : 0;
+                }
+                if (times) {
+                    atomicAdd(&cnt[t], (uint32_t)times);
+                    atomicOr(&bits[t >> 5], 1u << (t & 31));
+                }
+                if (ends_ngram(rr, ngram, base + k * LG_THREADS + (int)threadIdx.x)) atomicOr(&cnt[t], BANNED);
+            }
+        }
+        __syncthreads();
+    }
+};
+
 // The window's share of one thread: NV vectors of the row's 16-byte grid.
 // j0(v) is the vocabulary index of vector v's first element (it may be
 // negative, or the vector may end behind the row).
 template <typename T, int NV>
 struct Window {
     static constexpr int N = Vec<T>::N;
-    static constexpr int TOKENS = LG_THREADS * NV * N;
+    [[maybe_unused]] static constexpr int TOKENS = LG_THREADS * NV * N;
     int lo;  // vocabulary index of the window's first slot
     int vocab;
     __device__ __forceinline__ int slot(int v) const { return (v * LG_THREADS + (int)threadIdx.x) * N; }
     __device__ __forceinline__ int j0(int v) const { return lo + slot(v); }
     __device__ __forceinline__ bool whole(int v) const { return j0(v) >= 0 && j0(v) + N <= vocab; }
 
-    // logits as raw vectors; elements outside the row stay 0 and are skipped by every user
+    // logits as raw vectors; elements outside the row are -inf (whatever the rules make of them, they stay so)
+    __device__ __forceinline__ void load1(const T* row, int v, uint4& raw) const {
+        if (whole(v)) {
+            raw = __ldcs(reinterpret_cast<const uint4*>(row + j0(v)));
+        } else {
+            T part[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const int j = j0(v) + e;
+                part[e] = j >= 0 && j < vocab ? row[j] : T(-INFINITY);
+            }
+            memcpy(&raw, part, 16);
+        }
+    }
     __device__ __forceinline__ void load(const T* row, uint4 (&raw)[NV]) const {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            raw[v] = make_uint4(0, 0, 0, 0);
-            if (whole(v)) {
-                raw[v] = __ldcs(reinterpret_cast<const uint4*>(row + j0(v)));
-            } else {
-                T part[N];
+        for (int v = 0; v < NV; ++v) load1(row, v, raw[v]);
+    }
+    // The window's bias values and mask words, asked for before the history is counted. Through L1: where the bias row
+    // does not share the logits' 16-byte grid, eight neighbouring words come one by one from the same line (past L1 that
+    // was 8 times the traffic: 256 rows of 131071, 184 us).
+    struct Extra {
+        float bias[N];
+        uint32_t mask[2];
+    };
+    __device__ __forceinline__ void fetch(const RowRules& rr, int v, Extra& x) const {
+        if (rr.bias) {
+            const float* b = rr.bias + j0(v);
+            if (whole(v) && (reinterpret_cast<uintptr_t>(rr.bias + lo) & 15) == 0) {
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const int j = j0(v) + e;
-                    part[e] = j >= 0 && j < vocab ? row[j] : T(0.0f);
+                for (int e = 0; e < N; e += 4) {
+                    const float4 b4 = *reinterpret_cast<const float4*>(b + e);
+                    x.bias[e] = b4.x;
+                    x.bias[e + 1] = b4.y;
+                    x.bias[e + 2] = b4.z;
+                    x.bias[e + 3] = b4.w;
                 }
-                memcpy(&raw[v], part, 16);
-            }
-        }
-    }
-    // Counts the history's tokens of this window, and marks those that would complete an n-gram.
-    __device__ __forceinline__ void count(const RowRules& rr, int ngram, uint32_t* cnt) const {
-        for (int i = threadIdx.x; i < TOKENS / 4; i += LG_THREADS)
-            reinterpret_cast<uint4*>(cnt)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-        for (int i = threadIdx.x; i < rr.n_hist; i += LG_THREADS) {
-            const int id = rr.hist[i];
-            if (id < 0 || id >= vocab || id < lo || id - lo >= TOKENS) continue;
-            atomicAdd(&cnt[id - lo], 1u);
-            // token i ends an n-gram whose first ngram - 1 tokens are the history's last ones
-            if (ngram > 1 && i >= ngram - 1) {
-                bool same = true;
-                for (int e = 1; e < ngram && same; ++e) same = rr.hist[i - e] == rr.hist[rr.n_hist - e];
-                if (same) atomicOr(&cnt[id - lo], BANNED);
-            }
-        }
-        __syncthreads();
-    }
-    // The rules on vector v; `ok` has a bit for each element inside the row.
-    __device__ __forceinline__ void apply(const RowRules& rr, const uint32_t* cnt, bool counted, const uint4& raw, int v,
-                                          float (&x)[N], uint32_t& ok) const {
-        const int j = j0(v);
-        ok = 0;
+            } else if (whole(v)) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            x[e] = Vec<T>::get(raw, e);
-            ok |= (j + e >= 0 && j + e < vocab ? 1u : 0u) << e;
+                for (int e = 0; e < N; ++e) x.bias[e] = b[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e) x.bias[e] = j0(v) + e >= 0 && j0(v) + e < vocab ? b[e] : 0.0f;
+            }
         }
+        if (rr.mask) {
+            // bits j0 .. j0 + N - 1: they lie in one or two words
+            const int first = min(max(j0(v), 0), vocab - 1), last = min(max(j0(v) + N - 1, 0), vocab - 1);
+            x.mask[0] = rr.mask[first >> 5];
+            x.mask[1] = rr.mask[last >> 5];
+        }
+    }
+    // The rules on vector v.
+    template <int TABLE>
+    __device__ __forceinline__ void apply(const RowRules& rr, const History<TABLE>& hist, bool counted, const uint4& raw,
+                                          const Extra& extra, int v, float (&x)[N]) const {
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = Vec<T>::get(raw, e);
         uint32_t banned = 0;
         if (counted) {
-#pragma unroll
-            for (int e4 = 0; e4 < N; e4 += 4) {
-                const uint4 c4 = *reinterpret_cast<const uint4*>(cnt + slot(v) + e4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t c = (&c4.x)[e];
-                    if (c) {
-                        float y = x[e4 + e];
-                        y = y > 0.0f ? __fdiv_rn(y, rr.rep) : __fmul_rn(y, rr.rep);
-                        const float n = (float)(c & ~BANNED);
-                        x[e4 + e] = __fsub_rn(y, __fadd_rn(__fmul_rn(rr.freq, n), rr.pres));
-                        banned |= (c >> 31) << (e4 + e);
-                    }
-                }
-            }
-        }
-        if (rr.bias) {
-            const float* b = rr.bias + j;
-            if (ok == (1u << N) - 1 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
-#pragma unroll
-                for (int e4 = 0; e4 < N; e4 += 4) {
-                    const float4 b4 = __ldcg(reinterpret_cast<const float4*>(b + e4));
-                    x[e4] = __fadd_rn(x[e4], b4.x);
-                    x[e4 + 1] = __fadd_rn(x[e4 + 1], b4.y);
-                    x[e4 + 2] = __fadd_rn(x[e4 + 2], b4.z);
-                    x[e4 + 3] = __fadd_rn(x[e4 + 3], b4.w);
-                }
-            } else {
+            const int at = slot(v);
+            const uint32_t hit = (reinterpret_cast<const uint8_t*>(hist.bits)[at >> 3] >> (at & 7)) & ((1u << N) - 1);
+            if (hit) {
 #pragma unroll
                 for (int e = 0; e < N; ++e)
-                    if (ok >> e & 1) x[e] = __fadd_rn(x[e], __ldcg(b + e));
+                    if (hit & (1u << e)) {
+                        const uint32_t c = hist.cnt[at + e];
+                        x[e] = penalized(rr, x[e], c & ~BANNED);
+                        banned |= (c >> 31) << e;
+                    }
             }
         }
-        if (rr.mask && ok) {
-            // bits j .. j + N - 1: they lie in one or two words of the mask
-            const int first = j < 0 ? 0 : j, last = min(j + N, vocab) - 1;
-            const uint32_t w0 = __ldcg(rr.mask + (first >> 5)), w1 = __ldcg(rr.mask + (last >> 5));
-            const uint32_t bits = first >> 5 == last >> 5 ? w0 >> (first & 31) : __funnelshift_r(w0, w1, first & 31);
-            banned |= ~(bits << (first - j)) & ok;
-        }
+        finish(rr, extra, v, banned, x);
+    }
+    // Bias and mask, after the penalties; `banned` has a bit for each element that an n-gram excludes.
+    __device__ __forceinline__ void finish(const RowRules& rr, const Extra& extra, int v, uint32_t banned, float (&x)[N]) const {
+        const int j = j0(v);
+        if (rr.bias) {
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (banned >> e & 1) x[e] = -INFINITY;
+            for (int e = 0; e < N; ++e) x[e] = __fadd_rn(x[e], extra.bias[e]);
+        }
+        if (rr.mask) {
+            const int first = min(max(j, 0), vocab - 1), last = min(max(j + N - 1, 0), vocab - 1);
+            const uint32_t w0 = extra.mask[0], w1 = extra.mask[1];
+            const uint32_t bits = first >> 5 == last >> 5 ? w0 >> (first & 31) : __funnelshift_r(w0, w1, first & 31);
+            banned |= ~(bits << (first - j));  // (a bit of an element outside the row says nothing)
+        }
+        if (banned) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = banned & (1u << e) ? -INFINITY : x[e];
+        }
     }
 };
 
@@ -208,14 +278,17 @@ __global__ void __launch_bounds__(LG_THREADS) logits_process_kernel(const T* log
     uint4 raw[NV];
     w.load(in, raw);
     const RowRules rr(R, row);
+    typename W::Extra extra[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) w.fetch(rr, v, extra[v]);
     const bool counted = rr.n_hist > 0;
-    if (counted) w.count(rr, R.ngram, lg_cnt);
+    History<W::TOKENS> hist;
+    if (counted) hist.count(rr, R.ngram, lg_cnt, w.lo, vocab);
     const bool same_grid = ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(to)) & 15) == 0;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         float x[W::N];
-        uint32_t ok;
-        w.apply(rr, lg_cnt, counted, raw[v], v, x, ok);
+        w.apply(rr, hist, counted, raw[v], extra[v], v, x);
         if (same_grid && w.whole(v)) {
             T part[W::N];
 #pragma unroll
@@ -226,7 +299,7 @@ __global__ void __launch_bounds__(LG_THREADS) logits_process_kernel(const T* log
         } else {
 #pragma unroll
             for (int e = 0; e < W::N; ++e)
-                if (ok >> e & 1) store1(to + w.j0(v) + e, x[e]);
+                if (w.j0(v) + e >= 0 && w.j0(v) + e < vocab) store1(to + w.j0(v) + e, x[e]);
         }
     }
 }
@@ -248,251 +321,329 @@ __device__ __forceinline__ float cand_value(uint64_t c) { return from_order((uin
 __device__ __forceinline__ int cand_index(uint64_t c) { return (int)~(uint32_t)c; }
 
 struct Select {
-    uint64_t cand[CAND];    // the candidates; the first `kept` are the best so far, in order
+    uint64_t cand[CAND + 2];    // the candidates; the first `kept` are the best so far, in order
     uint64_t next[TOPK_MAX];
-    float tmax[LG_THREADS];
     float red[2 * (LG_THREADS / 32)];
-    int n, flag;
-    float bound;            // values at or below it cannot be among the k best any more
+    int n;
 };
 
-// Keeps the k best of the n candidates, in order, and raises the bound: each
+// Keeps the k best of the n candidates, in order: each
 // thread counts how many candidates beat its own.
 __device__ __forceinline__ void select_prune(Select& s, int k) {
     __syncthreads();
     const int n = s.n;
+    if (threadIdx.x == 0) s.cand[n] = 0;
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += LG_THREADS) {
         const uint64_t me = s.cand[i];
         int rank = 0;
-        for (int o = 0; o < n; ++o) rank += s.cand[o] > me;
+#pragma unroll 4
+        for (int o = 0; o < n; o += 2) {  // (behind the last one lies a 0: it beats none)
+            const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(s.cand + o);
+            rank += (c.x > me) + (c.y > me);
+        }
         if (rank < k) s.next[rank] = me;
     }
     __syncthreads();
     const int kept = min(n, k);
     for (int i = threadIdx.x; i < kept; i += LG_THREADS) s.cand[i] = s.next[i];
-    if (threadIdx.x == 0) {
-        s.n = kept;
-        if (kept == k) s.bound = cand_value(s.next[k - 1]);
-    }
+    if (threadIdx.x == 0) s.n = kept;
     __syncthreads();
 }
 
-// The k-th largest of the threads' own maxima: at least k values of the block
-// reach it.
-__device__ __forceinline__ float select_kth_max(Select& s, float mine, int k) {
-    s.tmax[threadIdx.x] = mine;
-    if (threadIdx.x == 0) s.red[0] = -INFINITY;
-    __syncthreads();
-    int above = 0, equal_before = 0;
-    const float4* t4 = reinterpret_cast<const float4*>(s.tmax);
-    for (int o = 0; o < LG_THREADS / 4; ++o) {
-        const float4 t = t4[o];
-        above += (t.x > mine) + (t.y > mine) + (t.z > mine) + (t.w > mine);
-        const int b = 4 * o;
-        equal_before += (t.x == mine && b < (int)threadIdx.x) + (t.y == mine && b + 1 < (int)threadIdx.x) +
-                        (t.z == mine && b + 2 < (int)threadIdx.x) + (t.w == mine && b + 3 < (int)threadIdx.x);
-    }
-    if (above + equal_before == k - 1) s.red[0] = mine;
-    __syncthreads();
-    const float r = s.red[0];
-    __syncthreads();
-    return r;
-}
-
-// One block works on windows first, first + step, ... of a row and leaves its
-// k best candidates, the largest value and the sum of exp(x - largest); the
-// last block of the row to finish joins them.
+// The selection's first pass: the rules on one window of a row, and what is left of it: the largest value of each
+// segment (one 16-byte step of a warp: 32 * N tokens) and the sum of exp(x - largest) of each warp.
 template <typename T, int NV>
 __global__ void __launch_bounds__(LG_THREADS)
-    logits_topk_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Rules R, int k, int windows_per_block,
-                       uint64_t* part, float2* part_ms, unsigned* done, int32_t* __restrict__ ids,
-                       float* __restrict__ logprob) {
+    logits_stats_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Rules R, float* __restrict__ seg_max,
+                        float* __restrict__ warp_sums) {
     pdl_entry();
     using W = Window<T, NV>;
     extern __shared__ __align__(16) uint32_t lg_cnt[];
-    __shared__ __align__(16) Select s;
-    const int row = blockIdx.y, n_part = gridDim.x;
+    const int row = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const T* in = logits + (int64_t)row * ld;
     const int shift = (int)(reinterpret_cast<uintptr_t>(in) / sizeof(T) % W::N);
+    W w;
+    w.vocab = vocab;
+    w.lo = (int)blockIdx.x * W::TOKENS - shift;
+    uint4 raw[NV];
+    w.load(in, raw);
     const RowRules rr(R, row);
+    typename W::Extra extra[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) w.fetch(rr, v, extra[v]);
     const bool counted = rr.n_hist > 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    if (threadIdx.x == 0) {
-        s.n = 0;
-        s.bound = -INFINITY;
-    }
-    float m = -INFINITY, sum = 0.0f;  // of this thread's values
-    constexpr float L2E = 1.4426950408889634f;
-    const int n_windows = (vocab + shift + W::TOKENS - 1) / W::TOKENS;
-    const int w0 = (int)blockIdx.x * windows_per_block, w1 = min(n_windows, w0 + windows_per_block);
-    __syncthreads();
-    for (int wi = w0; wi < w1; ++wi) {
-        W w;
-        w.vocab = vocab;
-        w.lo = wi * W::TOKENS - shift;
-        uint4 raw[NV];
-        w.load(in, raw);
-        if (counted) w.count(rr, R.ngram, lg_cnt);
-        float x[NV][W::N];
+    History<W::TOKENS> hist;
+    if (counted) hist.count(rr, R.ngram, lg_cnt, w.lo, vocab);
+    float x[NV][W::N];
+    float most = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+        w.apply(rr, hist, counted, raw[v], extra[v], v, x[v]);
         float mine = -INFINITY;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            uint32_t ok;
-            w.apply(rr, lg_cnt, counted, raw[v], v, x[v], ok);
-#pragma unroll
-            for (int e = 0; e < W::N; ++e) {
-                // outside the row, or not a number: never chosen and no part of the sum
-                if (!(ok >> e & 1) || !(x[v][e] == x[v][e])) x[v][e] = -INFINITY;
-                mine = fmaxf(mine, x[v][e]);
-            }
+        for (int e = 0; e < W::N; ++e) {
+            x[v][e] = fmaxf(x[v][e], -INFINITY);  // not a number: never chosen and no part of the sum
+            mine = fmaxf(mine, x[v][e]);
         }
-        // the running sum of exp(x - m); a largest value of +inf counts the values that reach it
-        if (mine > m) {
-            sum = m == -INFINITY || mine == INFINITY ? 0.0f : sum * exp2f((m - mine) * L2E);
-            m = mine;
-        }
-        if (m == INFINITY) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int e = 0; e < W::N; ++e) sum += x[v][e] == INFINITY ? 1.0f : 0.0f;
-        } else if (m > -INFINITY) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int e = 0; e < W::N; ++e) sum += exp2f((x[v][e] - m) * L2E);
-        }
-        // candidates: values above the bound. Windows ascend, so a value equal to the k-th best
-        // has the higher index and loses.
-        float bound = s.bound;
-        int have = s.n;
-        auto found = [&](bool at_bound) {  // how many of this window are above (or at) the bound
-            int c = 0;
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int e = 0; e < W::N; ++e) c += at_bound ? x[v][e] >= bound : x[v][e] > bound;
-            return c;
-        };
-        auto block_count = [&](int c) {
-            if (threadIdx.x == 0) s.flag = 0;
-            __syncthreads();
-            c = __reduce_add_sync(0xffffffffu, c);
-            if (lane == 0 && c) atomicAdd(&s.flag, c);
-            __syncthreads();
-            return s.flag;
-        };
-        if (!__syncthreads_or(mine > bound)) continue;
-        bool at_bound = false;
-        int c = block_count(found(false));
-        if (have + c > CAND) {
-            // too many (the first window, as a rule): the k-th largest of the threads' maxima bounds them
-            const float kth = select_kth_max(s, mine, k);
-            if (kth > bound) {
-                bound = kth;
-                at_bound = true;
-                c = block_count(found(true));
-            }
-        }
-        if (have + c <= CAND) {
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int e = 0; e < W::N; ++e)
-                    if (at_bound ? x[v][e] >= bound : x[v][e] > bound) {
-                        const int at = atomicAdd(&s.n, 1);
-                        s.cand[at] = cand_key(x[v][e], w.j0(v) + e);
-                    }
-            select_prune(s, k);
-        } else {
-            // many equal values: the window's best one after another, k times at most
-            uint64_t below = ~0ull;
-            for (int round = 0; round < k; ++round) {
-                uint64_t best = 0;
-#pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int e = 0; e < W::N; ++e) {
-                        const uint64_t me = cand_key(x[v][e], w.j0(v) + e);
-                        if (x[v][e] > -INFINITY && me < below && me > best) best = me;
-                    }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-                    best = other > best ? other : best;
-                }
-                if (lane == 0) s.next[warp] = best;
-                __syncthreads();
-                if (threadIdx.x == 0) {
-                    for (int o = 1; o < LG_THREADS / 32; ++o) best = s.next[o] > best ? s.next[o] : best;
-                    s.next[0] = best;
-                    if (best) s.cand[s.n++] = best;
-                }
-                __syncthreads();
-                below = s.next[0];
-                __syncthreads();
-                if (!below) break;
-            }
-            select_prune(s, k);
-        }
+        mine = from_order(__reduce_max_sync(0xffffffffu, order_bits(mine)));
+        most = fmaxf(most, mine);
+        if (lane == 0) seg_max[((int64_t)row * gridDim.x + blockIdx.x) * NV * WARPS + v * WARPS + warp] = mine;
     }
-    // the block's largest value and sum
-    {
-        const float bm = warp_max(m);
-        float bs = m == -INFINITY ? 0.0f : m == bm ? sum : bm == INFINITY ? 0.0f : sum * exp2f((m - bm) * L2E);
-        bs = warp_sum(bs);
-        if (lane == 0) {
-            s.red[warp] = bm;
-            s.red[LG_THREADS / 32 + warp] = bs;
-        }
+    float sum = 0.0f;
+    if (most == INFINITY) {  // +inf shares its probability among the values that reach it
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < W::N; ++e) sum += x[v][e] == INFINITY ? 1.0f : 0.0f;
+    } else if (most > -INFINITY) {
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int e = 0; e < W::N; ++e) sum += ex2((x[v][e] - most) * L2E);  // (not one fma: most * log2(e) would be rounded)
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) warp_sums[((int64_t)row * gridDim.x + blockIdx.x) * WARPS + warp] = sum;
+}
+
+// The second pass, one block a row: a value that the k best reach from the segments' largest values, then the few
+// segments that reach it once more, a warp each. Segments ascend with the tokens.
+template <typename T, int NV>
+__global__ void __launch_bounds__(LG_THREADS)
+    logits_pick_kernel(const T* __restrict__ logits, int64_t ld, int vocab, Rules R, int k, int windows,
+                       const float* __restrict__ seg_max, const float* __restrict__ warp_sums, int32_t* __restrict__ ids,
+                       float* __restrict__ logprob) {
+    pdl_entry();
+    constexpr int N = Vec<T>::N, SEG = 32 * N;
+    __shared__ __align__(16) Select s;
+    extern __shared__ __align__(16) uint32_t lg_hash[];  // [2][HASH]: token + 1 (0: none), how often it occurs
+    uint32_t *keys = lg_hash, *counts = lg_hash + HASH;
+    __shared__ uint32_t cnt_s[WARPS][SEG];
+    __shared__ int list_s[LG_THREADS];
+    __shared__ int list_n[WARPS];
+    const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const T* in = logits + (int64_t)row * ld;
+    const int shift = (int)(reinterpret_cast<uintptr_t>(in) / sizeof(T) % N);
+    const RowRules rr(R, row);
+    const int n_warp = windows * WARPS, n_seg = n_warp * NV;
+    const float* maxima = seg_max + (int64_t)row * n_seg;
+    const float* sums = warp_sums + (int64_t)row * n_warp;
+    // The history as a table (open addressing): what a look-up finds does not depend on the order of the inserts. One that
+    // is longer than half the table is counted anew for each segment.
+    const bool hashed = rr.n_hist > 0 && rr.n_hist <= HASH / 2;
+    auto slot_of = [](uint32_t t) { return (t * 2654435761u) >> (32 - HASH_BITS); };
+    if (hashed) {
+        for (int i = threadIdx.x; i < HASH / 2; i += LG_THREADS) reinterpret_cast<uint4*>(lg_hash)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
+        for (int base = 0; base < rr.n_hist; base += LG_THREADS) {
+            const int i = base + (int)threadIdx.x, id = i < rr.n_hist ? rr.hist[i] : -1;
+            const bool here = id >= 0 && id < vocab;
+            const unsigned with = __ballot_sync(0xffffffffu, here);
+            if (!here) continue;
+            const unsigned same = __match_any_sync(with, id);
+            const bool ends = ends_ngram(rr, R.ngram, i);
+            if (lane != __ffs(same) - 1 && !ends) continue;
+            uint32_t at = slot_of((uint32_t)id);
+            for (int probe = 0; probe < HASH; ++probe, at = (at + 1) & (HASH - 1)) {
+                const uint32_t was = atomicCAS(&keys[at], 0u, (uint32_t)id + 1);
+                if (was == 0 || was == (uint32_t)id + 1) break;
+            }
+            if (lane == __ffs(same) - 1) atomicAdd(&counts[at], (uint32_t)__popc(same));
+            if (ends) atomicOr(&counts[at], BANNED);
+        }
+    } else if (rr.n_hist) {
+        for (int i = lane; i < SEG; i += 32) cnt_s[warp][i] = 0;
     }
-    auto join = [&](float am, float as, float& M, float& S) {  // (M, S) += (am, as)
+    if (threadIdx.x == 0) s.n = 0;
+
+    // the row's largest value and sum, in a fixed order
+    float M = -INFINITY, S = 0.0f;
+    auto join = [&](float am, float as) {  // (M, S) += (am, as)
         if (am == -INFINITY) return;
         if (am > M) {
-            S = M == -INFINITY || am == INFINITY ? 0.0f : S * exp2f((M - am) * L2E);
+            S = M == -INFINITY || am == INFINITY ? 0.0f : S * ex2((M - am) * L2E);
             M = am;
         }
-        S += am == M ? as : M == INFINITY ? 0.0f : as * exp2f((am - M) * L2E);
+        S += am == M ? as : M == INFINITY ? 0.0f : as * ex2((am - M) * L2E);
     };
-    float M = -INFINITY, S = 0.0f;
-    for (int o = 0; o < LG_THREADS / 32; ++o) join(s.red[o], s.red[LG_THREADS / 32 + o], M, S);
-    if (n_part > 1) {
-        const int64_t p = (int64_t)row * n_part + blockIdx.x;
-        for (int i = threadIdx.x; i < k; i += LG_THREADS) part[p * k + i] = i < s.n ? s.cand[i] : 0ull;
-        if (threadIdx.x == 0) part_ms[p] = make_float2(M, S);
-        __threadfence();
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const unsigned before = atomicAdd(&done[row], 1u);
-            s.flag = before == (unsigned)n_part - 1;
-            if (s.flag) done[row] = 0;  // ready for the next call
+#pragma unroll 2
+    for (int i = threadIdx.x; i < n_warp; i += LG_THREADS) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) m = fmaxf(m, __ldcg(maxima + (i / WARPS * NV + v) * WARPS + i % WARPS));
+        join(m, __ldcg(sums + i));
+    }
+    // The bound: what k segments' largest values reach, to the first 16 bits of their order (more would not spare a
+    // segment often); with fewer than k segments above -inf, all of them.
+    float bound = -INFINITY;
+    {
+        constexpr int KEPT = 4;  // of a thread's segments, in registers
+        uint32_t key[KEPT];
+#pragma unroll
+        for (int i = 0; i < KEPT; ++i) {
+            const int g = i * LG_THREADS + (int)threadIdx.x;
+            key[i] = g < n_seg ? order_bits(__ldcg(maxima + g)) : 0;
         }
-        __syncthreads();
-        if (!s.flag) return;
-        __threadfence();
-        // the row's last block: joins the parts in order (the sum does not depend on who came last)
-        M = -INFINITY;
-        S = 0.0f;
-        for (int o = 0; o < n_part; ++o) {
-            const float2 ms = __ldcg(&part_ms[(int64_t)row * n_part + o]);
-            join(ms.x, ms.y, M, S);
-        }
-        if (threadIdx.x == 0) {
-            s.n = 0;
-            s.bound = -INFINITY;
-        }
-        __syncthreads();
-        const uint64_t* all = part + (int64_t)row * n_part * k;
-        const int total = n_part * k, room = CAND - k;
-        for (int c0 = 0; c0 < total; c0 += room) {
-            for (int i = c0 + threadIdx.x; i < min(total, c0 + room); i += LG_THREADS) {
-                const uint64_t c = __ldcg(all + i);
-                if (c) s.cand[atomicAdd(&s.n, 1)] = c;
+        uint32_t prefix = 0;
+        for (int bit = 31; bit >= 16; --bit) {
+            const uint32_t at_least = prefix | 1u << bit;
+            int reach = 0;
+#pragma unroll
+            for (int i = 0; i < KEPT; ++i)
+                if (i * LG_THREADS < n_seg) reach += __syncthreads_count(key[i] >= at_least);
+            for (int base = KEPT * LG_THREADS; base < n_seg && reach < k; base += LG_THREADS) {
+                const int g = base + (int)threadIdx.x;
+                reach += __syncthreads_count(g < n_seg && order_bits(__ldcg(maxima + g)) >= at_least);
             }
-            select_prune(s, k);
+            if (reach >= k) prefix = at_least;
+        }
+        if (prefix > order_bits(-INFINITY)) bound = from_order(prefix);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float om = __shfl_xor_sync(0xffffffffu, M, o), os = __shfl_xor_sync(0xffffffffu, S, o);
+        join(om, os);
+    }
+    __syncthreads();
+    if (lane == 0) {
+        s.red[warp] = M;
+        s.red[WARPS + warp] = S;
+    }
+    __syncthreads();
+    M = -INFINITY;
+    S = 0.0f;
+    for (int o = 0; o < WARPS; ++o) join(s.red[o], s.red[WARPS + o]);
+
+    bool exact = false;  // the bound is the k-th best so far: only what exceeds it matters, for it would lose a tie
+    // a value that is wanted; -inf never is
+    auto wanted = [&](float x) { return exact ? x > bound : x >= bound && x > -INFINITY; };
+
+    // segment g by one warp
+    auto scan = [&](int g) {
+        const int j = g * SEG + lane * N - shift;
+        Window<T, 1> w;
+        w.vocab = vocab;
+        w.lo = j - (int)threadIdx.x * N;  // (the window whose vector 0 is this one)
+        uint4 raw;
+        w.load1(in, 0, raw);
+        typename Window<T, 1>::Extra extra;
+        w.fetch(rr, 0, extra);
+        float x[N];
+        bool ban[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            x[e] = Vec<T>::get(raw, e);
+            ban[e] = false;
+        }
+        if (hashed) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint32_t key = (uint32_t)(j + e) + 1;
+                uint32_t at = slot_of(key - 1), k0 = keys[at];
+                while (k0 != 0 && k0 != key) k0 = keys[at = (at + 1) & (HASH - 1)];  // (half of the table is empty)
+                if (k0 == key) {
+                    const uint32_t c = counts[at];
+                    x[e] = penalized(rr, x[e], c & ~BANNED);
+                    ban[e] = c & BANNED;
+                }
+            }
+        } else if (rr.n_hist) {
+            uint32_t* cnt = cnt_s[warp];
+            const int lo = g * SEG - shift;
+            for (int base = 0; base < rr.n_hist; base += 128) {
+                int id[4];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int i = base + 32 * q + lane;
+                    id[q] = i < rr.n_hist ? rr.hist[i] : -1;
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const bool here = id[q] >= 0 && id[q] < vocab && id[q] >= lo && id[q] - lo < SEG;
+                    const unsigned with = __ballot_sync(0xffffffffu, here);
+                    if (!here) continue;
+                    const unsigned same = __match_any_sync(with, id[q]);
+                    if (lane == __ffs(same) - 1) atomicAdd(&cnt[id[q] - lo], (uint32_t)__popc(same));
+                    if (ends_ngram(rr, R.ngram, base + 32 * q + lane)) atomicOr(&cnt[id[q] - lo], BANNED);
+                }
+            }
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const uint32_t c = cnt[lane * N + e];
+                if (c) {
+                    x[e] = penalized(rr, x[e], c & ~BANNED);
+                    ban[e] = c & BANNED;
+                    cnt[lane * N + e] = 0;
+                }
+            }
+            __syncwarp();
+        }
+        uint32_t banned = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) banned |= (ban[e] ? 1u : 0u) << e;
+        w.finish(rr, extra, 0, banned, x);
+        uint32_t hit = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) hit |= (wanted(x[e]) ? 1u : 0u) << e;
+        if (hit) {
+            int at = atomicAdd(&s.n, __popc(hit));  // what there is no room for is only counted
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (hit & (1u << e)) {
+                    if (at < CAND) s.cand[at] = cand_key(x[e], j + e);
+                    ++at;
+                }
+        }
+    };
+    auto prune = [&] {
+        select_prune(s, k);
+        if (s.n == k) {
+            bound = cand_value(s.cand[k - 1]);
+            exact = true;
+        }
+    };
+
+    for (int g0 = 0; g0 < n_seg; g0 += LG_THREADS) {
+        // the segments of these that reach the bound, in order
+        const int g = g0 + (int)threadIdx.x;
+        const bool take = g < n_seg && wanted(__ldcg(maxima + g));
+        const unsigned takers = __ballot_sync(0xffffffffu, take);
+        __syncthreads();
+        if (lane == 0) list_n[warp] = __popc(takers);
+        __syncthreads();
+        int at = __popc(takers & ((1u << lane) - 1)), n_list = 0;
+        for (int o = 0; o < WARPS; ++o) {
+            if (o < warp) at += list_n[o];
+            n_list += list_n[o];
+        }
+        if (take) list_s[at] = g;
+        __syncthreads();
+        constexpr int ROUND = 2 * WARPS;
+        for (int i = 0; i < n_list; i += ROUND) {
+            const int have = s.n;  // (at rest: a barrier lies behind its last change)
+            __syncthreads();
+#pragma unroll
+            for (int o = 0; o < ROUND; o += WARPS)
+                if (i + o + warp < n_list) scan(list_s[i + o + warp]);
+            __syncthreads();
+            const int n = s.n;
+            __syncthreads();
+            if (n > CAND) {
+                // many equal values: one segment after another, which always fits, the bound rising as soon as it can
+                if (threadIdx.x == 0) s.n = have;
+                __syncthreads();
+                for (int o = 0; o < ROUND && i + o < n_list; ++o) {
+                    if (warp == o % WARPS) scan(list_s[i + o]);
+                    prune();
+                }
+            } else if (n >= PRUNE_AT) {
+                prune();
+            }
         }
     }
+    static_assert(PRUNE_AT + SEG <= CAND && TOPK_MAX < PRUNE_AT, "one segment more always fits");
+    prune();
     const float lse = logf(S);
     for (int i = threadIdx.x; i < k; i += LG_THREADS) {
         const bool have = i < s.n;
@@ -542,21 +693,29 @@ void check_logits(const vkb_context* ctx, const void* logits, int dtype, int64_t
         fail(VKB_ERROR_INVALID_ARGUMENT, "logits: misaligned logits");
 }
 
-constexpr int64_t ROWS_PER_LAUNCH = 32768;  // grid.y, and the arrival counters of a selection
+// 16-byte vectors of a thread: 4096 tokens a window either way. Half of that or twice it: process, 128 rows of 51866
+// (f32): 17.2 us, 4 vectors 15.0; select, 256 rows of 131071 (f16): 1 vector 153 us, 2 139, 4 358 (35 KB of counts).
+constexpr int NV_F32 = 4, NV_F16 = 2;
+constexpr int64_t ROWS_PER_LAUNCH = 32768;  // grid.y
+
+// The rules of the rows from r0 on.
+Rules rows_from(Rules R, int64_t r0) {
+    if (R.hist) R.hist += r0 * R.hist_ld;
+    for (const int32_t** p : {&R.hist_len, &R.bias_row, &R.mask_row})
+        if (*p) *p += r0;
+    for (const float** p : {&R.rep, &R.freq, &R.pres})
+        if (*p) *p += r0;
+    return R;
+}
 
 template <typename T, int NV>
 void launch_process(vkb_context* ctx, const T* in, int64_t ld, int64_t n_rows, int vocab, const Rules& R0, T* out,
                     int64_t out_ld) {
     using W = Window<T, NV>;
     const unsigned windows = (unsigned)ceil_div((int64_t)vocab + W::N - 1, W::TOKENS);
-    const size_t smem = R0.hist ? W::TOKENS * sizeof(uint32_t) : 0;
+    const size_t smem = R0.hist ? History<W::TOKENS>::BYTES : 0;
     for (int64_t r0 = 0; r0 < n_rows; r0 += ROWS_PER_LAUNCH) {
-        Rules R = R0;
-        if (R.hist) R.hist += r0 * R.hist_ld;
-        for (const int32_t** p : {&R.hist_len, &R.bias_row, &R.mask_row})
-            if (*p) *p += r0;
-        for (const float** p : {&R.rep, &R.freq, &R.pres})
-            if (*p) *p += r0;
+        const Rules R = rows_from(R0, r0);
         const unsigned rows = (unsigned)std::min<int64_t>(ROWS_PER_LAUNCH, n_rows - r0);
         launch_pdl(ctx, logits_process_kernel<T, NV>, dim3(windows, rows), LG_THREADS, smem, in + r0 * ld, ld, vocab, R,
                    out + r0 * out_ld, out_ld);
@@ -570,32 +729,20 @@ void launch_topk(vkb_context* ctx, const T* in, int64_t ld, int64_t n_rows, int 
                  int32_t* ids, float* logprob) {
     using W = Window<T, NV>;
     const int64_t windows = ceil_div((int64_t)vocab + W::N - 1, W::TOKENS);
-    const size_t smem = R0.hist ? W::TOKENS * sizeof(uint32_t) : 0;
+    const size_t smem = R0.hist ? History<W::TOKENS>::BYTES : 0;
     for (int64_t r0 = 0; r0 < n_rows; r0 += ROWS_PER_LAUNCH) {
-        Rules R = R0;
-        if (R.hist) R.hist += r0 * R.hist_ld;
-        for (const int32_t** p : {&R.hist_len, &R.bias_row, &R.mask_row})
-            if (*p) *p += r0;
-        for (const float** p : {&R.rep, &R.freq, &R.pres})
-            if (*p) *p += r0;
+        const Rules R = rows_from(R0, r0);
         const int64_t rows = std::min<int64_t>(ROWS_PER_LAUNCH, n_rows - r0);
-        // blocks of a row: enough for four on each SM, at most one a window
-        const int64_t want = std::max<int64_t>(1, (4 * (int64_t)ctx->sm_count + rows - 1) / rows);
-        const int64_t per = (windows + std::min(want, windows) - 1) / std::min(want, windows);
-        const int64_t parts = (windows + per - 1) / per;
-        uint64_t* part = nullptr;
-        float2* part_ms = nullptr;
-        if (parts > 1) {
-            const size_t cand = (size_t)(rows * parts * k) * sizeof(uint64_t);
-            ctx->ensure_workspace(cand + (size_t)(rows * parts) * sizeof(float2));
-            part = ctx->workspace.as<uint64_t>();
-            part_ms = reinterpret_cast<float2*>(ctx->workspace.as<uint8_t>() + cand);
-        }
-        launch_pdl(ctx, logits_topk_kernel<T, NV>, dim3((unsigned)parts, (unsigned)rows), LG_THREADS, smem, in + r0 * ld,
-                   ld, vocab, R, k, (int)per, part, part_ms, ctx->tile_ctr.as<unsigned>(), ids + r0 * k,
-                   logprob + r0 * k);
+        const size_t maxima = (size_t)(rows * windows * NV * WARPS), sums = (size_t)(rows * windows * WARPS);
+        ctx->ensure_workspace((maxima + sums) * sizeof(float));
+        float* ws = ctx->workspace.as<float>();
+        launch_pdl(ctx, logits_stats_kernel<T, NV>, dim3((unsigned)windows, (unsigned)rows), LG_THREADS, smem, in + r0 * ld,
+                   ld, vocab, R, ws, ws + maxima);
+        smem_optin(logits_pick_kernel<T, NV>, 2 * HASH * (int)sizeof(uint32_t));
+        launch_pdl(ctx, logits_pick_kernel<T, NV>, dim3((unsigned)rows), LG_THREADS, R0.hist ? 2 * HASH * sizeof(uint32_t) : 0, in + r0 * ld, ld, vocab, R, k,
+                   (int)windows, ws, ws + maxima, ids + r0 * k, logprob + r0 * k);
         VKB_CUDA(cudaGetLastError());
-        ctx->count();
+        ctx->count(2);
     }
 }
 
@@ -620,10 +767,10 @@ vkb_status vkb_logits_process(vkb_context* ctx, const void* logits_dev, int32_t 
         NvtxRange nvtx_range("vkb.logits.process");
         const int v = (int)n_vocab;
         if (dtype == VKB_DT_F32)
-            launch_process<float, 4>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R,
+            launch_process<float, NV_F32>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R,
                                      reinterpret_cast<float*>(out_dev), out_ld);
         else
-            launch_process<__half, 4>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R,
+            launch_process<__half, NV_F16>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R,
                                       reinterpret_cast<__half*>(out_dev), out_ld);
     });
 }
@@ -640,10 +787,10 @@ vkb_status vkb_logits_topk(vkb_context* ctx, const void* logits_dev, int32_t dty
         NvtxRange nvtx_range("vkb.logits.topk");
         const int v = (int)n_vocab;
         if (dtype == VKB_DT_F32)
-            launch_topk<float, 4>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
+            launch_topk<float, NV_F32>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
                                   logprob_dev);
         else
-            launch_topk<__half, 4>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
+            launch_topk<__half, NV_F16>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
                                    logprob_dev);
     });
 }
