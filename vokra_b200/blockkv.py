@@ -19,16 +19,17 @@ from __future__ import annotations
 
 import ctypes as C
 
+import torch
+
 from . import _lib
 from ._lib import check, VkbError  # noqa: F401
-from .logits import _bad, _tensor
+from .logits import _DTYPES, _bad, _tensor
 
 _L = _lib.load()
 BLOCK = _lib.BKV_BLOCK
 
 
 def _i32(t, name, ndim):
-    import torch
     if t is None:
         _bad(f"{name}: missing")
     return _tensor(t, name, (torch.int32,), ndim)
@@ -74,7 +75,6 @@ class PageState:
     @staticmethod
     def empty(n_seq: int, max_pages: int, n_pages: int, device="cuda") -> "PageState":
         """Streams without tokens."""
-        import torch
         return PageState(torch.full((n_seq, max_pages), -1, dtype=torch.int32, device=device),
                          torch.zeros(n_seq, dtype=torch.int32, device=device),
                          torch.zeros(n_pages, dtype=torch.int32, device=device))
@@ -131,7 +131,6 @@ class BlockKvCache:
     d_head, 16] and their scales f32 [n_layer, n_pages, n_kv_head]; d_head 32, 64, 96, 128 or 256."""
 
     def __init__(self, ctx, k, v, k_scale, v_scale):
-        import torch
         _tensor(k, "k", (torch.int8,), 5)
         _tensor(v, "v", (torch.int8,), 5)
         n_layer, n_pages, n_kv_head, block, d_head = k.shape
@@ -151,7 +150,6 @@ class BlockKvCache:
 
     @staticmethod
     def empty(ctx, n_layer: int, n_kv_head: int, d_head: int, n_pages: int) -> "BlockKvCache":
-        import torch
         dev = f"cuda:{ctx.device}"
         k = torch.zeros(n_layer, n_pages, n_kv_head, BLOCK, d_head, dtype=torch.int8, device=dev)
         v = torch.zeros(n_layer, n_pages, n_kv_head, d_head, BLOCK, dtype=torch.int8, device=dev)
@@ -164,20 +162,17 @@ class BlockKvCache:
 
     def _rows(self, t, name, heads, batch):
         """(pointer, row stride, dtype code) of rows [n_tok, heads, d_head] or [n_tok, heads * d_head]."""
-        import torch
-        if t.dtype == torch.float16:
-            dt = _lib.DT_F16
-        elif t.dtype == torch.float32:
-            dt = _lib.DT_F32
-        else:
+        dt = _DTYPES.get(t.dtype)
+        if dt is None:
             _bad(f"{name}: f32 or f16 rows are wanted, got {t.dtype}")
-        width = heads * self.d_head
-        ok = t.is_cuda and (t.dim() == 2 and t.shape[1] == width and (width == 1 or t.stride(1) == 1) or
-                            t.dim() == 3 and t.shape[1:] == (heads, self.d_head) and t.stride(2) == 1 and
-                            (heads == 1 or t.stride(1) == self.d_head))
-        if not ok or t.shape[0] < batch.n_tok:
-            _bad(f"{name}: CUDA rows [{batch.n_tok}, {heads}, {self.d_head}] with contiguous rows are wanted, got {tuple(t.shape)}")
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width, dt
+        shape, stride, d = t.shape, t.stride(), self.d_head
+        if len(shape) == 3:
+            ok = shape[1] == heads and shape[2] == d and stride[2] == 1 and (stride[1] == d or heads == 1)
+        else:
+            ok = len(shape) == 2 and shape[1] == heads * d and stride[1] == 1
+        if not ok or shape[0] < batch.n_tok or not t.is_cuda:
+            _bad(f"{name}: CUDA rows [{batch.n_tok}, {heads}, {d}] with contiguous rows are wanted, got {tuple(shape)}")
+        return t.data_ptr(), stride[0] if shape[0] > 1 else heads * d, dt
 
     def append(self, layer: int, batch: Batch, k, v):
         """Stores the batch's rows of k and v ([n_tok, n_kv_head, d_head], f32 or f16, any row stride)."""
@@ -185,27 +180,33 @@ class BlockKvCache:
         vp, v_ld, dt_v = self._rows(v, "v", self.n_kv_head, batch)
         if dt != dt_v:
             _bad("k and v must have the same type")
-        check(_L.vkb_bkv_append(self.ctx.h, self.ref, layer, batch.ref, kp, k_ld, vp, v_ld, dt))
+        status = _L.vkb_bkv_append(self.ctx.h, self.ref, layer, batch.ref, kp, k_ld, vp, v_ld, dt)
+        if status:
+            check(status)
 
     def attention(self, layer: int, batch: Batch, q, scale: float = 1.0, out=None):
         """Causal attention of the rows q [n_tok, n_head, d_head] over their streams' caches; out like q unless given."""
-        import torch
         heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.d_head
         qp, q_ld, q_dt = self._rows(q, "q", heads, batch)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        op, o_ld, o_dt = self._rows(out, "out", heads, batch)
-        check(_L.vkb_bkv_attention(self.ctx.h, self.ref, layer, batch.ref, heads, qp, q_ld, q_dt, scale, op, o_ld, o_dt))
+            op, o_ld, o_dt = out.data_ptr(), heads * self.d_head, q_dt
+        else:
+            op, o_ld, o_dt = self._rows(out, "out", heads, batch)
+        status = _L.vkb_bkv_attention(self.ctx.h, self.ref, layer, batch.ref, heads, qp, q_ld, q_dt, scale, op, o_ld, o_dt)
+        if status:
+            check(status)
         return out
 
     def read(self, layer: int, batch: Batch, dtype=None):
         """(k, v): the stored values of the streams' last rows, [n_tok, n_kv_head, d_head], f32 or f16."""
-        import torch
         dtype = dtype or torch.float32
-        if dtype not in (torch.float32, torch.float16):
+        dt = _DTYPES.get(dtype)
+        if dt is None:
             _bad(f"read: dtype must be f32 or f16, got {dtype}")
-        k = torch.empty(batch.n_tok, self.n_kv_head, self.d_head, dtype=dtype, device=self.k.device)
+        k = torch.empty((batch.n_tok, self.n_kv_head, self.d_head), dtype=dtype, device=self.k.device)
         v = torch.empty_like(k)
-        check(_L.vkb_bkv_read(self.ctx.h, self.ref, layer, batch.ref, k.data_ptr(), v.data_ptr(),
-                              _lib.DT_F16 if dtype == torch.float16 else _lib.DT_F32))
+        status = _L.vkb_bkv_read(self.ctx.h, self.ref, layer, batch.ref, k.data_ptr(), v.data_ptr(), dt)
+        if status:
+            check(status)
         return k, v

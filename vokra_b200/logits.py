@@ -15,6 +15,8 @@ from __future__ import annotations
 
 import ctypes as C
 
+import torch
+
 from . import _lib
 from ._lib import check, VkbError  # noqa: F401
 
@@ -56,7 +58,6 @@ class LogitsRules:
 
     def __init__(self, history=None, history_len=None, repetition=None, frequency=None, presence=None,
                  no_repeat_ngram: int = 0, bias=None, bias_row=None, mask=None, mask_row=None):
-        import torch
         i32, f32 = (torch.int32,), (torch.float32,)
         self.tensors = (history, history_len, repetition, frequency, presence, bias, bias_row, mask, mask_row)
         s = _lib.LogitsRules()
@@ -100,46 +101,61 @@ class LogitsRules:
         self._checked = (rows, vocab)
 
 
-def _logits(logits, name: str):
-    import torch
-    p = _tensor(logits, name, (torch.float32, torch.float16), 2)
-    return p, _lib.DT_F16 if logits.dtype == torch.float16 else _lib.DT_F32
+_DTYPES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16}
+
+
+def _matrix(t, name: str):
+    """(pointer, dtype code, rows, columns, row stride) of an f32 or f16 CUDA matrix with contiguous rows."""
+    dt = _DTYPES.get(t.dtype)
+    if dt is None or not t.is_cuda or t.dim() != 2:
+        _tensor(t, name, tuple(_DTYPES), 2)
+    rows, cols = t.shape
+    ld, unit = t.stride()
+    if unit != 1 and cols > 1:
+        _bad(f"{name}: its last axis must be contiguous")
+    return t.data_ptr(), dt, rows, cols, ld if rows > 1 else cols
 
 
 def process(ctx, logits, rules: LogitsRules | None = None, out=None):
     """The logits ([rows, vocab], f32 or f16) after the rules, in their own type; out may be logits."""
-    import torch
-    p, dt = _logits(logits, "logits")
-    rows, vocab = logits.shape
+    p, dt, rows, vocab, ld = _matrix(logits, "logits")
     if out is None:
-        out = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+        out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
+        to, out_ld = out.data_ptr(), vocab
     else:
-        _logits(out, "out")
-        if out.shape != logits.shape or out.dtype != logits.dtype:
+        to, out_dt, out_rows, out_vocab, out_ld = _matrix(out, "out")
+        if (out_rows, out_vocab, out_dt) != (rows, vocab, dt):
             _bad("out: another shape or dtype than logits")
+    ref = None
     if rules is not None:
-        rules.check(rows, vocab)
-    check(_L.vkb_logits_process(ctx.h, p, dt, rows, vocab, _ld(logits), rules.ref if rules else None, out.data_ptr(), _ld(out)))
+        if rules._checked != (rows, vocab):
+            rules.check(rows, vocab)
+        ref = rules.ref
+    status = _L.vkb_logits_process(ctx.h, p, dt, rows, vocab, ld, ref, to, out_ld)
+    if status:
+        check(status)
     return out
 
 
 def topk(ctx, logits, k: int, rules: LogitsRules | None = None, ids=None, logprobs=None):
     """(ids int32 [rows, k], log-probabilities f32 [rows, k]) of the k best tokens after the rules, the
     best first, ties by the lower id; id -1 at -inf where fewer than k tokens are left."""
-    import torch
-    p, dt = _logits(logits, "logits")
-    rows, vocab = logits.shape
+    p, dt, rows, vocab, ld = _matrix(logits, "logits")
     if not 1 <= k <= TOPK_MAX:
         _bad(f"k must be in 1..{TOPK_MAX}, got {k}")
-    if ids is None:
-        ids = torch.empty(rows, k, dtype=torch.int32, device=logits.device)
-    if logprobs is None:
-        logprobs = torch.empty(rows, k, dtype=torch.float32, device=logits.device)
     for t, name, dtype in ((ids, "ids", torch.int32), (logprobs, "logprobs", torch.float32)):
-        if t.dtype != dtype or tuple(t.shape) != (rows, k) or not t.is_contiguous() or not t.is_cuda:
+        if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows, k) or not t.is_contiguous() or not t.is_cuda):
             _bad(f"{name}: a contiguous {dtype} CUDA tensor of shape [{rows}, {k}] is wanted")
+    if ids is None:
+        ids = torch.empty((rows, k), dtype=torch.int32, device=logits.device)
+    if logprobs is None:
+        logprobs = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
+    ref = None
     if rules is not None:
-        rules.check(rows, vocab)
-    check(_L.vkb_logits_topk(ctx.h, p, dt, rows, vocab, _ld(logits), rules.ref if rules else None, k, ids.data_ptr(),
-                             logprobs.data_ptr()))
+        if rules._checked != (rows, vocab):
+            rules.check(rows, vocab)
+        ref = rules.ref
+    status = _L.vkb_logits_topk(ctx.h, p, dt, rows, vocab, ld, ref, k, ids.data_ptr(), logprobs.data_ptr())
+    if status:
+        check(status)
     return ids, logprobs
