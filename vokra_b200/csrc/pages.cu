@@ -15,7 +15,9 @@ namespace {
 
 constexpr int PT = 256;     // threads of the wide kernels
 constexpr int PLAN = 1024;  // threads of the planning block
-constexpr int COPY_BYTES = 32 * 1024;  // bytes of a page that one block moves
+constexpr int COPY_BYTES = 64 * 1024;  // bytes of a page that one block moves: at half of that the loads of a thread in flight
+                                       // were one (33 KB a page and layer, 34000 pages: 524 us)
+constexpr int CHUNK = 4 * PLAN;        // pages that a planning block looks at
 
 struct Planes {
     int n_layer, n;
@@ -40,7 +42,7 @@ struct Pool {
 struct Plan {
     int32_t* info;
     int32_t* base;    // [n_seq] length after the fork
-    int32_t* first;   // [n_seq] the stream's first entry of `fresh`
+    int32_t* first;   // [n_seq] the stream's first entry of `fresh`; compaction: pages in use of each chunk
     int2* copy;       // [n_seq] (source, destination) of a stream's copied page, or (-1, -1)
     int32_t* fresh;   // [n_pages] free pages in order; compaction: destinations
     int32_t* moved;   // [n_pages] compaction: sources
@@ -228,16 +230,16 @@ __device__ __forceinline__ void move_page(const Planes& A, int layer, int64_t sr
         const int64_t n = A.page[p] / A.unit[p];
         const int64_t lo = n * part / parts, hi = n * (part + 1) / parts;
         if (A.unit[p] == 16) {
-            constexpr int U = 4;
-            int64_t i = lo + threadIdx.x;
-            for (; i + (U - 1) * PT < hi; i += U * PT) {
+            constexpr int U = 8;
+            for (int64_t i = lo + threadIdx.x; i < hi; i += U * PT) {
                 uint4 v[U];
 #pragma unroll
-                for (int u = 0; u < U; ++u) v[u] = __ldcs(reinterpret_cast<const uint4*>(from) + i + u * PT);
+                for (int u = 0; u < U; ++u)
+                    if (i + u * PT < hi) v[u] = __ldcs(reinterpret_cast<const uint4*>(from) + i + u * PT);
 #pragma unroll
-                for (int u = 0; u < U; ++u) __stcs(reinterpret_cast<uint4*>(to) + i + u * PT, v[u]);
+                for (int u = 0; u < U; ++u)
+                    if (i + u * PT < hi) __stcs(reinterpret_cast<uint4*>(to) + i + u * PT, v[u]);
             }
-            for (; i < hi; i += PT) reinterpret_cast<uint4*>(to)[i] = reinterpret_cast<const uint4*>(from)[i];
         } else if (A.unit[p] == 4) {
             for (int64_t i = lo + threadIdx.x; i < hi; i += PT)
                 reinterpret_cast<uint32_t*>(to)[i] = reinterpret_cast<const uint32_t*>(from)[i];
@@ -263,48 +265,74 @@ __global__ void __launch_bounds__(PT) pages_copy_kernel(Pool P, Planes A, State 
     for (int j = blockIdx.x; j < A.n_layer * parts; j += gridDim.x) move_page(A, j / parts, c.x, c.y, j % parts, parts);
 }
 
-// One block: the pages in use, and which of them go where.
+// Pages in use of each chunk.
+__global__ void __launch_bounds__(PLAN) compact_count_kernel(Pool P, const int32_t* __restrict__ refs, Plan W) {
+    pdl_entry();
+    int used = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t i = (int64_t)blockIdx.x * CHUNK + e * PLAN + threadIdx.x;
+        used += __syncthreads_count(i < P.n_pages && refs[i] > 0);
+    }
+    if (threadIdx.x == 0) W.first[blockIdx.x] = used;
+}
+
+// One block a chunk: which of its pages are holes before the number in use, and which are in use behind it. The place of
+// each in its list is a count of pages in use: holes before page i are i - used(i), moves before it used(i) - used(n).
 __global__ void __launch_bounds__(PLAN) compact_plan_kernel(Pool P, const int32_t* __restrict__ refs, Plan W, int32_t* n_used) {
     pdl_entry();
-    const int t = threadIdx.x;
-    int used = 0;
-    for (int64_t i = t; i < P.n_pages; i += PLAN) used += refs[i] > 0;
-    int total;
-    block_scan(used, total);
-    used = total;
-    int holes = 0, moves = 0;
-    for (int64_t i0 = 0; i0 < P.n_pages; i0 += 4 * PLAN) {
-        int pick = 0, nh = 0, nm = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t i = i0 + 4 * t + e;
-            if (i >= P.n_pages) continue;
-            const bool live = refs[i] > 0;
-            if (i < used ? !live : live) {
-                pick |= 1 << e;
-                if (i < used) ++nh;
-                else ++nm;
-            }
-        }
-        int th, tm;
-        int h = holes + block_scan(nh, th), m = moves + block_scan(nm, tm);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (pick >> e & 1) {
-                const int64_t i = i0 + 4 * t + e;
-                if (i < used) W.fresh[h++] = (int)i;
-                else {
-                    W.map[i] = m;
-                    W.moved[m++] = (int)i;
-                }
-            }
-        holes += th;
-        moves += tm;
+    const int t = threadIdx.x, chunks = gridDim.x, me = blockIdx.x;
+    __shared__ int before_s, total_s;
+    if (t == 0) before_s = total_s = 0;
+    __syncthreads();
+    for (int c = t; c < chunks; c += PLAN) {
+        const int u = W.first[c];
+        atomicAdd(&total_s, u);
+        if (c < me) atomicAdd(&before_s, u);
     }
-    if (t == 0) {
-        W.info[1] = moves;
-        W.info[2] = used;
-        if (n_used) *n_used = used;
+    __syncthreads();
+    const int n = total_s;  // pages in use: they become pages 0 .. n - 1
+    // used(n): whole chunks before n, and the part of the one that n lies in
+    __shared__ int below_s;
+    if (t == 0) below_s = 0;
+    __syncthreads();
+    const int at = n / CHUNK;
+    for (int c = t; c < at; c += PLAN) atomicAdd(&below_s, W.first[c]);
+    int part = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t i = (int64_t)at * CHUNK + e * PLAN + t;
+        part += __syncthreads_count(i < n && refs[i] > 0);
+    }
+    __syncthreads();
+    const int below = below_s + part;
+    int live = 0, mine = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t i = (int64_t)me * CHUNK + 4 * t + e;
+        if (i < P.n_pages && refs[i] > 0) {
+            live |= 1 << e;
+            ++mine;
+        }
+    }
+    int total;
+    int used = before_s + block_scan(mine, total);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int64_t i = (int64_t)me * CHUNK + 4 * t + e;
+        if (i >= P.n_pages) break;
+        const bool in_use = live >> e & 1;
+        if (i < n && !in_use) W.fresh[i - used] = (int)i;
+        if (i >= n && in_use) {
+            W.map[i] = used - below;
+            W.moved[used - below] = (int)i;
+        }
+        used += in_use;
+    }
+    if (me == 0 && t == 0) {
+        W.info[1] = n - below;
+        W.info[2] = n;
+        if (n_used) *n_used = n;
     }
 }
 
@@ -378,7 +406,7 @@ void check_states(const Pool& P, const vkb_page_state* a, const vkb_page_state* 
 }
 
 Plan make_plan(vkb_context* ctx, const Pool& P) {
-    const size_t seq = ((size_t)P.n_seq + 3) & ~(size_t)3, pages = ((size_t)P.n_pages + 3) & ~(size_t)3;
+    const size_t seq = ((size_t)std::max<int64_t>(P.n_seq, P.n_pages / CHUNK + 1) + 3) & ~(size_t)3, pages = ((size_t)P.n_pages + 3) & ~(size_t)3;
     ctx->ensure_workspace((16 + 4 * seq + 3 * pages) * 4);
     int32_t* w = ctx->workspace.as<int32_t>();
     Plan W;
@@ -440,10 +468,12 @@ vkb_status vkb_pages_compact(vkb_context* ctx, const vkb_page_pool* pool, const 
         NvtxRange nvtx_range("vkb.pages.compact");
         const Plan W = make_plan(ctx, P);
         const State a = state_of(from), b = state_of(to);
-        launch_pdl(ctx, compact_plan_kernel, dim3(1), PLAN, 0, P, a.refs, W, n_used_dev);
+        const unsigned chunks = (unsigned)((P.n_pages + CHUNK - 1) / CHUNK);
+        launch_pdl(ctx, compact_count_kernel, dim3(chunks), PLAN, 0, P, a.refs, W);
+        launch_pdl(ctx, compact_plan_kernel, dim3(chunks), PLAN, 0, P, a.refs, W, n_used_dev);
         launch_pdl(ctx, compact_move_kernel, dim3((unsigned)(8 * ctx->sm_count)), PT, 0, P, A, a, b, W, page_parts(A));
         VKB_CUDA(cudaGetLastError());
-        ctx->count(2);
+        ctx->count(3);
     });
 }
 
