@@ -463,7 +463,18 @@ void launch(vkb_context* ctx, const BkvAttn& a) {
 bool bkv_prompt_takes(const vkb_context* ctx, const BkvAttn& a) {
     if (!a.q_f16 || !a.out_f16 || (a.d_head != 64 && a.d_head != 128)) return false;
     if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_ld % 8 || a.out_ld % 8) return false;
-    return (int64_t)a.max_q * a.group >= 64 && (int64_t)a.S.n_tok * a.group / ROWS * a.L.n_kv_head >= 16;
+    // A wave of these blocks takes the time of its longest stream whatever the rows; the other kernel's grows with the
+    // rows and less with the keys. Microseconds here and there, 8 KV heads of 128, group 4, one stream:
+    //   500 keys, 16 rows 16 and 23; 64 rows 20 and 25          (tables of up to 32 pages: here)
+    //   1000 keys, 32 rows 27 and 25; 64 rows 29 and 34         (64 and 128 tiles of 16 rows, all heads)
+    //   2000 keys, 64 rows 49 and 41; 128 rows 50 and 54        (128 and 256 tiles)
+    //   4000 keys, 128 rows 87 and 73; 256 rows 88 and 115      (256 and 512 tiles)
+    // 8 heads of 64, 1000 keys: 64 tiles 25 and 22, 128 tiles 26 and 29; 20 heads, 2000 keys: 320 tiles 45 and 41.
+    if ((int64_t)a.max_q * a.group < 64) return false;
+    if (a.S.ld <= 32) return true;
+    const int64_t blocks = most_tiles(a) * a.L.n_kv_head, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
+    const int64_t tiles = ((int64_t)a.S.n_tok * a.group + 15) / 16 * a.L.n_kv_head;
+    return tiles >= waves * a.S.ld * (a.d_head == 64 ? 5 : 3) / 2;
 }
 
 void run_bkv_prompt(vkb_context* ctx, const BkvAttn& a) {
