@@ -14,6 +14,12 @@ without reading anything back. The definitions are in include/vkb200.h
     for layer in range(n_layer):
         cache.append(layer, step, k, v)
         out = cache.attention(layer, step, q, scale)
+
+The context's stream is the one that was torch's current stream when the context
+was made (Context.set_stream changes it). Tensors that were written, or are read
+or freed, on another stream are ordered by the caller, with an event, as for any
+other kernel; a tensor that a call allocates belongs to torch's current stream.
+A whole decode loop is in examples/beam_decode.py.
 """
 from __future__ import annotations
 

@@ -9,7 +9,8 @@ include/vkb200.h (vkb_logits_rules).
 
 Tensors are torch CUDA tensors and stay the caller's: a rules object keeps them
 alive and reads what they hold when a call runs, so a program makes it once and
-updates the tensors in place. The work runs on the context's stream.
+updates the tensors in place. The work runs on the context's stream; tensors of
+another stream are ordered by the caller, as for any other kernel.
 """
 from __future__ import annotations
 
