@@ -99,3 +99,56 @@ def test_pages_that_run_out(ctx):
     model = bd.Decoder(ctx, vocab=259, d_model=64, n_layer=1, n_head=2, n_kv_head=1, d_head=32)
     with pytest.raises(VkbError, match="exhausted"):
         bd.beam_search(model, [[9, 8, 7]], 4, 20, 0, n_pages=2)
+
+
+def test_a_step_in_a_graph(ctx):
+    """A recorded step reads tables, lengths, counts, history and masks when it runs."""
+    import torch
+    from vokra_b200 import logits, ops
+    from vokra_b200.blockkv import Batch, BlockKvCache, PageState
+    n_seq, heads, group, d, vocab, n_pages, ld = 3, 2, 4, 64, 999, 64, 8
+    rng = np.random.default_rng(3)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        own = ops.Context(0)
+        status = torch.zeros(1, dtype=torch.int32, device="cuda")
+        k, v = (torch.zeros(n_seq, heads, d, device="cuda", dtype=torch.float16) for _ in range(2))
+        q = torch.zeros(n_seq, heads * group, d, device="cuda", dtype=torch.float16)
+        x = torch.zeros(n_seq, vocab, device="cuda")
+        history = torch.zeros(n_seq, 6, dtype=torch.int32, device="cuda")
+        rules = logits.LogitsRules(history=history, frequency=torch.ones(n_seq, device="cuda"))
+        parent = torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+        one = torch.ones(n_seq, dtype=torch.int32, device="cuda")
+        start = torch.arange(n_seq + 1, dtype=torch.int32, device="cuda")
+        y, ids, lp = torch.empty_like(q), torch.empty(n_seq, 4, dtype=torch.int32, device="cuda"), torch.empty(n_seq, 4, device="cuda")
+
+        def world():
+            cache = BlockKvCache.empty(own, 1, heads, d, n_pages)
+            return cache, cache.pages(status), PageState.empty(n_seq, ld, n_pages), PageState.empty(n_seq, ld, n_pages)
+
+        def step(cache, pages, a, b):
+            pages.advance(a, b, parent, one)
+            batch = Batch(start, b.len, b.table, n_seq, 1, status)
+            cache.append(0, batch, k, v)
+            cache.attention(0, batch, q, 0.125, out=y)
+            logits.topk(own, x, 4, rules, ids=ids, logprobs=lp)
+            for s, t in ((b.table, a.table), (b.len, a.len), (b.refs, a.refs)):
+                t.copy_(s)
+
+        recorded, eager = world(), world()
+        step(*world())  # sizes the scratch
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step(*recorded)
+    with torch.cuda.stream(stream):
+        for i in range(40):
+            for t in (k, v, q, x):
+                t.copy_(torch.from_numpy(rng.standard_normal(t.shape).astype(np.float32)))
+            history.copy_(torch.from_numpy(rng.integers(0, vocab, (n_seq, 6)).astype(np.int32)))
+            parent.copy_(torch.from_numpy(rng.integers(0, n_seq, n_seq).astype(np.int32)))
+            graph.replay()
+            got = [t.clone() for t in (y, ids, lp)]
+            step(*eager)
+            assert all(torch.equal(g, t) for g, t in zip(got, (y, ids, lp))), i
+    assert int(status) == 0 and int(recorded[2].len[0]) == 40
