@@ -120,6 +120,8 @@ struct History {
     __device__ __forceinline__ void count(const RowRules& rr, int ngram, uint32_t* smem, int lo, int vocab) {
         cnt = smem;
         bits = smem + TOKENS;
+        const int first = max(lo, 0);
+        const uint32_t width = (uint32_t)max(0, min(lo + TOKENS, vocab) - first);
         int id[4];
         auto fetch = [&](int base) {
 #pragma unroll
@@ -136,7 +138,7 @@ struct History {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const int t = id[k] - lo;
-                const bool here = id[k] >= 0 && id[k] < vocab && t >= 0 && t < TOKENS;
+                const bool here = (uint32_t)id[k] - (uint32_t)first < width;
                 const unsigned with = __ballot_sync(0xffffffffu, here);
                 if (!here) continue;
                 int times = 1;
@@ -229,15 +231,19 @@ struct Window {
         uint32_t banned = 0;
         if (counted) {
             const int at = slot(v);
-            const uint32_t hit = (reinterpret_cast<const uint8_t*>(hist.bits)[at >> 3] >> (at & 7)) & ((1u << N) - 1);
-            if (hit) {
+            uint32_t hit = (reinterpret_cast<const uint8_t*>(hist.bits)[at >> 3] >> (at & 7)) & ((1u << N) - 1);
+            // one element of a lane at a time, so that lanes with one hit each, at whatever place, take one turn together
+            while (hit) {
+                const int which = __ffs(hit) - 1;
+                hit &= hit - 1;
+                float y = x[0];
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (hit & (1u << e)) {
-                        const uint32_t c = hist.cnt[at + e];
-                        x[e] = penalized(rr, x[e], c & ~BANNED);
-                        banned |= (c >> 31) << e;
-                    }
+                for (int e = 1; e < N; ++e) y = which == e ? x[e] : y;
+                const uint32_t c = hist.cnt[at + which];
+                y = penalized(rr, y, c & ~BANNED);
+                banned |= (c >> 31) << which;
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[e] = which == e ? y : x[e];
             }
         }
         finish(rr, extra, v, banned, x);
@@ -250,9 +256,8 @@ struct Window {
             for (int e = 0; e < N; ++e) x[e] = __fadd_rn(x[e], extra.bias[e]);
         }
         if (rr.mask) {
-            const int first = min(max(j, 0), vocab - 1), last = min(max(j + N - 1, 0), vocab - 1);
-            const uint32_t w0 = extra.mask[0], w1 = extra.mask[1];
-            const uint32_t bits = first >> 5 == last >> 5 ? w0 >> (first & 31) : __funnelshift_r(w0, w1, first & 31);
+            const int first = min(max(j, 0), vocab - 1);
+            const uint32_t bits = __funnelshift_r(extra.mask[0], extra.mask[1], first & 31);
             banned |= ~(bits << (first - j));  // (a bit of an element outside the row says nothing)
         }
         if (banned) {
@@ -369,38 +374,41 @@ __global__ void __launch_bounds__(LG_THREADS)
     uint4 raw[NV];
     w.load(in, raw);
     const RowRules rr(R, row);
-    typename W::Extra extra[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) w.fetch(rr, v, extra[v]);
+    typename W::Extra extra;
+    w.fetch(rr, 0, extra);
     const bool counted = rr.n_hist > 0;
     History<W::TOKENS> hist;
     if (counted) hist.count(rr, R.ngram, lg_cnt, w.lo, vocab);
-    float x[NV][W::N];
-    float most = -INFINITY;
+    // vector by vector: the sum is of exp(x - most), `most` the warp's largest value so far
+    float most = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-        w.apply(rr, hist, counted, raw[v], extra[v], v, x[v]);
-        float mine = -INFINITY;
+        float x[W::N];
+        w.apply(rr, hist, counted, raw[v], extra, v, x);
+        if (v + 1 < NV) w.fetch(rr, v + 1, extra);
+        float mine = -INFINITY;  // (fmaxf leaves out what is not a number)
 #pragma unroll
-        for (int e = 0; e < W::N; ++e) {
-            x[v][e] = fmaxf(x[v][e], -INFINITY);  // not a number: never chosen and no part of the sum
-            mine = fmaxf(mine, x[v][e]);
-        }
+        for (int e = 0; e < W::N; ++e) mine = fmaxf(mine, x[e]);
         mine = from_order(__reduce_max_sync(0xffffffffu, order_bits(mine)));
-        most = fmaxf(most, mine);
         if (lane == 0) seg_max[((int64_t)row * gridDim.x + blockIdx.x) * NV * WARPS + v * WARPS + warp] = mine;
-    }
-    float sum = 0.0f;
-    if (most == INFINITY) {  // +inf shares its probability among the values that reach it
+        const float before = most;
+        most = fmaxf(most, mine);
+        if (most == INFINITY) {  // +inf shares its probability among the values that reach it
+            if (before != INFINITY) sum = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+            for (int e = 0; e < W::N; ++e) sum += x[e] == INFINITY ? 1.0f : 0.0f;
+        } else if (most > -INFINITY) {
+            sum *= ex2((before - most) * L2E);
+            float part = 0.0f;
 #pragma unroll
-            for (int e = 0; e < W::N; ++e) sum += x[v][e] == INFINITY ? 1.0f : 0.0f;
-    } else if (most > -INFINITY) {
+            for (int e = 0; e < W::N; ++e) part += ex2((x[e] - most) * L2E);  // (not one fma: most * log2(e) would be rounded)
+            if (part != part) {  // something is not a number: it is never chosen and no part of the sum
+                part = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int e = 0; e < W::N; ++e) sum += ex2((x[v][e] - most) * L2E);  // (not one fma: most * log2(e) would be rounded)
+                for (int e = 0; e < W::N; ++e) part += x[e] == x[e] ? ex2((x[e] - most) * L2E) : 0.0f;
+            }
+            sum += part;
+        }
     }
     sum = warp_sum(sum);
     if (lane == 0) warp_sums[((int64_t)row * gridDim.x + blockIdx.x) * WARPS + warp] = sum;
@@ -693,9 +701,9 @@ void check_logits(const vkb_context* ctx, const void* logits, int dtype, int64_t
         fail(VKB_ERROR_INVALID_ARGUMENT, "logits: misaligned logits");
 }
 
-// 16-byte vectors of a thread: 4096 tokens a window either way. Half of that or twice it: process, 128 rows of 51866
-// (f32): 17.2 us, 4 vectors 15.0; select, 256 rows of 131071 (f16): 1 vector 153 us, 2 139, 4 358 (35 KB of counts).
-constexpr int NV_F32 = 4, NV_F16 = 2;
+// 16-byte vectors of a thread. process, 128 rows of 51866 (f32): 2 vectors 17.2 us, 4 15.6. Selection, 256 rows of
+// 131071 (f16): 2 vectors 108 us, 3 107, 4 104 (fewer looks at a history of 2048 tokens).
+constexpr int NV_F32 = 4, NV_F16 = 2, NV_TOPK = 4;
 constexpr int64_t ROWS_PER_LAUNCH = 32768;  // grid.y
 
 // The rules of the rows from r0 on.
@@ -787,10 +795,10 @@ vkb_status vkb_logits_topk(vkb_context* ctx, const void* logits_dev, int32_t dty
         NvtxRange nvtx_range("vkb.logits.topk");
         const int v = (int)n_vocab;
         if (dtype == VKB_DT_F32)
-            launch_topk<float, NV_F32>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
+            launch_topk<float, NV_TOPK>(ctx, reinterpret_cast<const float*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
                                   logprob_dev);
         else
-            launch_topk<__half, NV_F16>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
+            launch_topk<__half, NV_TOPK>(ctx, reinterpret_cast<const __half*>(logits_dev), ld, n_rows, v, R, k, ids_dev,
                                    logprob_dev);
     });
 }
