@@ -297,3 +297,23 @@ def test_refusals(ctx):
     assert L.vkb_logits_process(ctx.h, p + 2, _lib.DT_F32, 1, 10, 10, None, p, 10) == _lib.ERROR_INVALID_ARGUMENT
     assert L.vkb_logits_topk(ctx.h, None, _lib.DT_F32, 2, 100, 100, None, 1, p, p) == _lib.ERROR_INVALID_ARGUMENT
     assert L.vkb_logits_topk(None, p, _lib.DT_F32, 2, 100, 100, None, 1, p, p) == _lib.ERROR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("hist", [60, 2100])
+@pytest.mark.parametrize("what", ["repetition", "presence", "frequency"])
+def test_penalties_that_raise(ctx, dtype, hist, what):
+    """Penalties below their neutral value lift tokens into the k best."""
+    import torch
+    from vokra_b200 import logits
+    rng = np.random.default_rng(hist)
+    rows, vocab, k = 3, 5003, 9
+    x = (rng.standard_normal((rows, vocab)) - 3).astype(dtype)
+    kw = dict(history=rng.integers(0, vocab, (rows, hist)).astype(np.int32), no_repeat_ngram=2,
+              **{what: np.full(rows, 0.01 if what == "repetition" else -2.5, np.float32)})
+    ids, lp = logits.topk(ctx, torch.from_numpy(x).cuda(), k, rules_of(kw))
+    torch.cuda.synchronize()
+    y = plain_rules(x, vocab, **kw)
+    want, _ = plain_topk(y, k)
+    assert np.isin(want[0], kw["history"][0]).any()  # the case is what it says
+    check_topk(y, k, ids, lp)
