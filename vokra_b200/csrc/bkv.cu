@@ -11,10 +11,13 @@
 // IEEE fp32, so the stored bytes are defined to the bit. NaN counts as 0 and
 // infinities as the largest finite value of the block.
 //
-// Bound: HBM. One warp holds one block of one head and side: each lane owns
-// d_head / 32 neighbouring channels of all 16 tokens, so a token's row is one
-// coalesced load, the maximum is one warp reduction, and a V block goes out as
-// 16-byte stores without a transpose.
+// Bound: HBM, then the conversions. One warp holds one block of one head and
+// side: each lane owns d_head / 32 neighbouring channels of all 16 tokens, so a
+// token's row is one coalesced load, the maximum is one warp reduction, and a V
+// block goes out as 16-byte stores without a transpose. Measured, 8 streams with
+// about 8500 new tokens in all, 8 heads of 128, f16: append 27 us (52 MB: 1.9
+// TB/s), read as f32 15.7 us (87 MB: 5.5 TB/s). Rounding by a magic number with an integer
+// maximum, a branch for whole blocks, or a path of their own: 55, 42 and 29 us.
 #include "bkv.cuh"
 #include <cfloat>
 #include <algorithm>
