@@ -15,8 +15,9 @@
 // side: each lane owns d_head / 32 neighbouring channels of all 16 tokens, so a
 // token's row is one coalesced load, the maximum is one warp reduction, and a V
 // block goes out as 16-byte stores without a transpose. Measured, 8 streams with
-// about 8500 new tokens in all, 8 heads of 128, f16: append 27 us (52 MB: 1.9
-// TB/s), read as f32 15.7 us (87 MB: 5.5 TB/s). Rounding by a magic number with an integer
+// about 8500 new tokens in all, 8 heads of 128, f16: append 23.5 us (52 MB:
+// 2.2 TB/s; 27 with the rows asked for behind the page's id and the status), read
+// as f32 15.5 us (87 MB: 5.6 TB/s). Rounding by a magic number with an integer
 // maximum, a branch for whole blocks, or a path of their own: 55, 42 and 29 us.
 #include "bkv.cuh"
 #include <cfloat>
@@ -156,7 +157,7 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS)
     const int lane = threadIdx.x & 31;
     const int job = (int)blockIdx.x * APPEND_WARPS + (int)(threadIdx.x >> 5);
     if (job >= 2 * L.n_kv_head) return;
-    if (status && *status != 0) return;
+    const int refused = status ? *status : 0;  // (looked at behind the loads, which do not depend on it)
     const bool is_v = job >= L.n_kv_head;
     const int h = is_v ? job - L.n_kv_head : job;
     const int s = blockIdx.z;
@@ -168,24 +169,23 @@ __global__ void __launch_bounds__(32 * APPEND_WARPS)
     const int p_begin = max(pos0, 0) / BKV_BLOCK, p_end = (n_keys + BKV_BLOCK - 1) / BKV_BLOCK;
     for (int p = p_begin + (int)blockIdx.y; p < p_end; p += gridDim.y) {
         const int64_t id = S.page(s, p, L.n_pages);
-        if (id < 0) continue;
         const int t0 = max(pos0 - p * BKV_BLOCK, 0);                   // first new slot
         const int t1 = min(n_keys - p * BKV_BLOCK, BKV_BLOCK);         // behind the last one
+        const int64_t ld = is_v ? v_ld : k_ld;
+        const T* src = (is_v ? v : k) + (int64_t)(first_row + p * BKV_BLOCK - pos0) * ld + h * D + lane * C;
+        float x[BKV_BLOCK][C];
+#pragma unroll
+        for (int t = 0; t < BKV_BLOCK; ++t) load_row<T, C, VEC>(src + min(max(t, t0), t1 - 1) * ld, x[t]);
+        if (id < 0 || refused != 0) continue;
         const int64_t head = id * L.n_kv_head + h;
         float* sp = (is_v ? L.vs : L.ks) + head;
         int8_t* q = (is_v ? L.v : L.k) + head * (BKV_BLOCK * D);
-        const T* src = (is_v ? v : k) + (int64_t)(first_row + p * BKV_BLOCK - pos0) * (is_v ? v_ld : k_ld) + h * D + lane * C;
-        const int64_t ld = is_v ? v_ld : k_ld;
         const float s_old = t0 > 0 ? *sp : 0.0f;
-        float x[BKV_BLOCK][C];
-        float amax = 0.0f;
+        float amax = 0.0f;  // (a new row that stands in for another one changes nothing)
 #pragma unroll
         for (int t = 0; t < BKV_BLOCK; ++t)
-            if (t >= t0 && t < t1) {
-                load_row<T, C, VEC>(src + t * ld, x[t]);
 #pragma unroll
-                for (int c = 0; c < C; ++c) amax = fmaxf(amax, fabsf(x[t][c]));
-            }
+            for (int c = 0; c < C; ++c) amax = fmaxf(amax, fabsf(x[t][c]));
         amax = fminf(warp_max(amax), FLT_MAX);
         const float s_new = fmaxf(s_old, amax * SCALE);
         const float inv = s_new > 0.0f ? __fdiv_rn(1.0f, s_new) : 0.0f;
