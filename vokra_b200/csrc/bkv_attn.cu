@@ -259,63 +259,78 @@ __device__ __forceinline__ void store_pair(const AttnArgs& A, int64_t at, float 
     }
 }
 
-// Joins row r of `n` parts, in order, a warp a row; part i's rows are o(i) and their (max, sum) ml(i). To the
-// output, or (to_o) to another part.
+// Joins rows r and (if it is not negative) r2 of `n` parts, in order, a warp for both at once: their loads are one round
+// trip. Part i's rows are o(i) and their (max, sum) ml(i). To the output, or (to_o) to another part.
 template <int D, class FO, class FM>
-__device__ __forceinline__ void join_row(const AttnArgs& A, int n, int r, int64_t row_at, int tile_row0, int h, FO o, FM ml,
-                                         float* to_o, float2* to_ml) {
+__device__ __forceinline__ void join_rows(const AttnArgs& A, int n, int r, int r2, int64_t row_at, int tile_row0, int h, FO o,
+                                          FM ml, float* to_o, float2* to_ml) {
     const int lane = threadIdx.x & 31;
     constexpr int C = D / 32;  // channels of a lane, as pairs 64 apart (one alone for D = 32, three for D = 96)
-    float m = -INFINITY, l = 0.0f, y[C];
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, y[2][C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) y[i] = 0.0f;
+    for (int i = 0; i < 2 * C; ++i) y[i / C][i % C] = 0.0f;
     auto ch = [&](int i) { return C == 1 ? lane : C % 2 ? lane + 32 * i : 64 * (i / 2) + 2 * lane + i % 2; };
-    constexpr int U = C <= 4 ? 8 : 4;
+    // parts at a time: 2, 4, 8: 48 ragged streams 121, 123, 128 us; one of 131071 keys 60.9, 58.0, 58.7
+    constexpr int U = C <= 4 ? 4 : 2;
     for (int p0 = 0; p0 < n; p0 += U) {
-        float2 x[U];
-        float v[U][C];
+        float2 x[2][U];
+        float v[2][U][C];
 #pragma unroll
-        for (int p = 0; p < U; ++p) {
-            const bool real = p0 + p < n;
-            x[p] = real ? __ldcg(ml(p0 + p) + r) : make_float2(-INFINITY, 0.0f);
-            const float* row = o(real ? p0 + p : 0) + r * D;
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int p = 0; p < U; ++p) {
+                const bool real = p0 + p < n && (k == 0 || r2 >= 0);
+                const int rk = real && k ? r2 : r;
+                x[k][p] = real ? __ldcg(ml(p0 + p) + rk) : make_float2(-INFINITY, 0.0f);
+#pragma unroll
+                for (int i = 0; i < C; ++i) v[k][p][i] = 0.0f;
+                if (real) {
+                    const float* row = o(p0 + p) + rk * D;
+#pragma unroll
+                    for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
+                        if constexpr (C % 2) {
+                            v[k][p][i] = __ldcg(row + ch(i));
+                        } else {
+                            const float2 f = __ldcg(reinterpret_cast<const float2*>(row + ch(i)));
+                            v[k][p][i] = f.x;
+                            v[k][p][i + 1] = f.y;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int p = 0; p < U; ++p) {
+                const float m_new = fmaxf(m[k], x[k][p].x);
+                const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+                const float a = ex2(m[k] - m_use), b = ex2(x[k][p].x - m_use);
+                l[k] = l[k] * a + x[k][p].y * b;
+#pragma unroll
+                for (int i = 0; i < C; ++i) y[k][i] = y[k][i] * a + v[k][p][i] * b;
+                m[k] = m_new;
+            }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int rk = k ? r2 : r;
+        if (rk < 0) continue;
+        if (to_o) {
+#pragma unroll
+            for (int i = 0; i < C; ++i) to_o[rk * D + ch(i)] = y[k][i];
+            if (lane == 0) to_ml[rk] = make_float2(m[k], l[k]);
+        } else {
+            const int row = tile_row0 + rk, tok = row / A.group, head = h * A.group + row % A.group;
+            const float inv = l[k] == 0.0f ? 0.0f : 1.0f / l[k];
+            const int64_t at = (row_at + tok) * A.out_ld + (int64_t)head * D;
 #pragma unroll
             for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
                 if constexpr (C % 2) {
-                    v[p][i] = __ldcg(row + ch(i));
+                    if (A.out_f16) reinterpret_cast<__half*>(A.out)[at + ch(i)] = __float2half_rn(y[k][i] * inv);
+                    else reinterpret_cast<float*>(A.out)[at + ch(i)] = y[k][i] * inv;
                 } else {
-                    const float2 f = __ldcg(reinterpret_cast<const float2*>(row + ch(i)));
-                    v[p][i] = f.x;
-                    v[p][i + 1] = f.y;
+                    store_pair(A, at + ch(i), y[k][i] * inv, y[k][i + 1] * inv);
                 }
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < U; ++p) {
-            const float m_new = fmaxf(m, x[p].x);
-            const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-            const float a = ex2(m - m_use), b = ex2(x[p].x - m_use);
-            l = l * a + x[p].y * b;
-#pragma unroll
-            for (int i = 0; i < C; ++i) y[i] = y[i] * a + (p0 + p < n ? v[p][i] : 0.0f) * b;
-            m = m_new;
-        }
-    }
-    if (to_o) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) to_o[r * D + ch(i)] = y[i];
-        if (lane == 0) to_ml[r] = make_float2(m, l);
-    } else {
-        const int row = tile_row0 + r, tok = row / A.group, head = h * A.group + row % A.group;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const int64_t at = (row_at + tok) * A.out_ld + (int64_t)head * D;
-#pragma unroll
-        for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
-            if constexpr (C % 2) {
-                if (A.out_f16) reinterpret_cast<__half*>(A.out)[at + ch(i)] = __float2half_rn(y[i] * inv);
-                else reinterpret_cast<float*>(A.out)[at + ch(i)] = y[i] * inv;
-            } else {
-                store_pair(A, at + ch(i), y[i] * inv, y[i + 1] * inv);
             }
         }
     }
@@ -748,10 +763,13 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
             while (i / 2 + n < AW && parts[2 * (i / 2 + n)].chunks && parts[2 * (i / 2 + n)].u0 == p.u0) ++n;
             const int64_t to = ((int64_t)blockIdx.x * 2 + (i == 0 ? 0 : 1)) * TR;
             auto nth = [&](int j) { return ((int64_t)blockIdx.x * AW * 2 + (j ? 2 * (i / 2 + j) : i)) * TR; };
-            for (; job < rows; job += AW)
-                join_row<D>(A, n, job, st.first[p.s], p.tile * TR, p.h, [&](int j) { return A.warp_o + nth(j) * D; },
+            while (job < rows) {
+                const int second = job + AW < rows ? job + AW : -1;
+                join_rows<D>(A, n, job, second, st.first[p.s], p.tile * TR, p.h, [&](int j) { return A.warp_o + nth(j) * D; },
                             [&](int j) { return A.warp_ml + nth(j); }, whole ? nullptr : A.block_o + to * D,
                             whole ? nullptr : A.block_ml + to);
+                job += second < 0 ? AW : 2 * AW;
+            }
         }
         job -= rows;
     }
@@ -776,8 +794,8 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
         const int rows = min(TR, st.n_q[p.s] * A.group - p.tile * TR);
         // the item starts somewhere in its first block's range, and at the start of every other one's
         auto nth = [&](int b) { return ((first + b) * 2 + (b == 0 && p.u0 != first * total / n_block ? 1 : 0)) * TR; };
-        for (int r = warp; r < rows; r += AW)
-            join_row<D>(A, n, r, st.first[p.s], p.tile * TR, p.h, [&](int b) { return A.block_o + nth(b) * D; },
+        for (int r = warp; r < rows; r += 2 * AW)
+            join_rows<D>(A, n, r, r + AW < rows ? r + AW : -1, st.first[p.s], p.tile * TR, p.h, [&](int b) { return A.block_o + nth(b) * D; },
                         [&](int b) { return A.block_ml + nth(b); }, nullptr, nullptr);
     }
 }
