@@ -499,3 +499,23 @@ def test_refusals(ctx):
     assert L.vkb_bkv_append(ctx.h, None, 0, b.ref, None, 128, None, 128, 0) == _lib.ERROR_INVALID_ARGUMENT
     assert L.vkb_bkv_append(ctx.h, cache.ref, 0, b.ref, None, 128, None, 128, 0) == _lib.ERROR_INVALID_ARGUMENT
     assert L.vkb_bkv_read(ctx.h, cache.ref, 0, None, None, None, 0) == _lib.ERROR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("d,dtype,most", [(64, "float32", 3), (64, "float16", 3), (128, "float16", 9), (256, "float32", 2), (32, "float16", 9)])
+def test_many_short_streams_beside_long_ones(ctx, d, dtype, most):
+    """Several steps for every warp of the GPU: shares count an item's fixed cost, ends of shares fall anywhere, in an
+    item's last steps too; more streams than one launch takes."""
+    rng = np.random.default_rng(d + most)
+    heads, group, n_seq = 4, 2, 560
+    lens = rng.integers(0, 260, n_seq)
+    lens[[3, 250, 511, 540]] = [1500, 64, 2100, 1023]
+    lens[20:40] = 0
+    new = rng.integers(0, most + 1, n_seq)
+    new[100:130] = 0
+    start = np.concatenate([[0], np.cumsum(new)])
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    q = (rng.standard_normal((start[-1], heads * group, d)) * 0.5).astype(dtype)
+    out = cache_of(ctx, plain).attention(0, batch_of(table, start, lens), dev(q), d**-0.5)
+    want = plain.attention(table, start, lens, q, d**-0.5)
+    assert np.abs(out.cpu().numpy() - want).max() <= TOL[dtype]

@@ -29,7 +29,8 @@
 //
 // The (stream, KV head, row tile, 64 keys) steps of the whole call are one
 // sequence, cut into equal contiguous shares for the blocks and their warps, so
-// ragged lengths balance themselves. A warp finishes an item that lies in its
+// ragged lengths balance themselves (an item counts a few steps more than it has,
+// for its query rows and its join). A warp finishes an item that lies in its
 // share alone; parts of shared items are joined in order, first within the
 // block, then by the last block of the item to arrive.
 #include "bkv_attn.cuh"
@@ -112,6 +113,7 @@ struct Streams {
     int keys[BKV_SEQ_PER_LAUNCH];
     int first[BKV_SEQ_PER_LAUNCH];
     int n_q[BKV_SEQ_PER_LAUNCH];
+    int extra;  // steps that an item counts for beside its own
 };
 
 template <int D>
@@ -130,11 +132,14 @@ struct Ring {
 };
 
 template <int TR, int AW>
-__device__ __forceinline__ void load_streams(const AttnArgs& A, Streams& st) {
+__device__ __forceinline__ void load_streams(const AttnArgs& A, Streams& st, int extra) {
     __shared__ int64_t sums[AW];
     const int n = A.S.n_seq, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int64_t carry = 0;
-    if (threadIdx.x == 0) st.pre[0] = 0;
+    if (threadIdx.x == 0) {
+        st.pre[0] = 0;
+        st.extra = extra;
+    }
     for (int base = 0; base < n; base += 32 * AW) {
         const int s = base + (int)threadIdx.x;
         int64_t x = 0;
@@ -145,7 +150,7 @@ __device__ __forceinline__ void load_streams(const AttnArgs& A, Streams& st) {
             st.keys[s] = keys;
             st.first[s] = first;
             st.n_q[s] = rows;
-            x = (int64_t)A.L.n_kv_head * ((rows * A.group + TR - 1) / TR) * max(1, (keys + 63) / 64);
+            x = (int64_t)A.L.n_kv_head * ((rows * A.group + TR - 1) / TR) * (max(1, (keys + 63) / 64) + extra);
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -176,7 +181,7 @@ struct Walk {
 
     __device__ __forceinline__ void stream(const AttnArgs& A, const Streams& st) {
         tiles = (st.n_q[s] * A.group + TR - 1) / TR;
-        chunks = max(1, (st.keys[s] + 63) / 64);
+        chunks = max(1, (st.keys[s] + 63) / 64) + st.extra;
     }
     __device__ __forceinline__ void item(const AttnArgs& A, const Streams& st) {
         const int last_tok = min(st.n_q[s] * A.group, (tile + 1) * TR) - 1;
@@ -345,6 +350,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
     constexpr int NT = D / 8;                // channel tiles of P.V
     using R = Ring<D>;
     constexpr int AW = R::AW;
+    constexpr int EXTRA = SPLIT ? 1 : 3;
     extern __shared__ __align__(16) uint8_t smem[];
     Streams& st = *reinterpret_cast<Streams*>(smem);
     __shared__ Part parts[2 * AW];
@@ -358,8 +364,18 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
         ptx::fence_mbar_init();
     }
     if (lane < 2) parts[2 * warp + lane].chunks = 0;
-    load_streams<TR, AW>(A, st);
+    load_streams<TR, AW>(A, st, 0);
     __syncthreads();
+    // An item costs its query rows and its join too, as much as EXTRA steps. They are counted, behind its own steps, once
+    // there is a step for every warp; else short items gather in a few blocks. 48 ragged streams of up to 8191 keys, 16
+    // rows: 124 us without them (one block 250 thousand cycles, the others 150 to 210), 97 with 2 to 4; 256 streams of up
+    // to 448 keys, 8 rows: 80 us without, 62 with one, 64 with two. From two steps a warp on: 64 streams of up to 448 keys
+    // 28.8 -> 27.6, from one on also 8 streams of up to 2000 keys 19.6 -> 17.2.
+    if (st.pre[A.S.n_seq] >= (int64_t)AW * gridDim.x) {
+        __syncthreads();
+        load_streams<TR, AW>(A, st, EXTRA);
+        __syncthreads();
+    }
     const int64_t total = st.pre[A.S.n_seq];
     // Equal shares for the blocks and their warps. Few steps go to as many blocks, a warp in each, not to the warps of
     // few blocks: 5 streams of up to 100 keys, 20 heads of 64, 12.0 us instead of 15.9; one of up to 1000 keys, 8 heads
@@ -425,6 +441,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
             uint32_t qb[KW / 2][SPLIT ? 2 : 4];  // the third plane (SPLIT, 32-bit rows), or the second one of 16 rows
             float row_fac[NR];  // multiplies a score: scale * log2(e) * the units of the planes
             int limit[NR];      // keys that the row sees
+            if (c0 < c_last)
 #pragma unroll
             for (int half_row = 0; half_row < NR; ++half_row) {
                 const int r = tile * TR + half_row * 8 + g;
