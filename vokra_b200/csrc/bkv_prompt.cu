@@ -88,29 +88,33 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
     pdl_entry();
     using M = Smem<D>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // the block's row tile: number x of all streams' tiles, found by every warp for itself
+    // The block's row tile: number x of all streams' tiles, found by every warp for itself. Of each 32 streams those with
+    // the most keys come first, and of a stream its last tile, which sees the most: long blocks do not start last.
+    // 8 prompts of up to 512 tokens, up to 8000 keys: 264 us with the streams as they come, 227.
     const int h = (int)(blockIdx.x % A.L.n_kv_head);
     int x = (int)(blockIdx.x / A.L.n_kv_head), s = -1, first_row = 0, n_q = 0, tile = 0;
     for (int base = 0; base < A.S.n_seq && s < 0; base += 32) {
-        int first = 0, n = 0;
-        if (base + lane < A.S.n_seq) A.S.rows(base + lane, first, n);
+        const int here = min(32, A.S.n_seq - base);
+        int first = 0, n = 0, keys = 0;
+        if (lane < here) {
+            A.S.rows(base + lane, first, n);
+            keys = A.S.keys(base + lane);
+        }
         const int mine = (int)(((int64_t)n * A.group + ROWS - 1) / ROWS);
         int sum = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += y;
+        for (int o = 0; o < here; ++o) {
+            const int other = __shfl_sync(0xffffffffu, keys, o), tiles = __shfl_sync(0xffffffffu, mine, o);
+            if (other > keys || (other == keys && o < lane)) sum += tiles;
         }
-        const unsigned behind = __ballot_sync(0xffffffffu, sum > x);
-        if (behind) {
-            const int at = __ffs(behind) - 1;
+        const unsigned found = __ballot_sync(0xffffffffu, x >= sum - mine && x < sum);
+        if (found) {
+            const int at = __ffs(found) - 1;
             s = base + at;
             first_row = __shfl_sync(0xffffffffu, first, at);
             n_q = __shfl_sync(0xffffffffu, n, at);
-            // a stream's last tile sees the most keys: it comes first
             tile = __shfl_sync(0xffffffffu, sum, at) - 1 - x;
         } else {
-            x -= __shfl_sync(0xffffffffu, sum, 31);
+            x -= __reduce_add_sync(0xffffffffu, mine);
         }
     }
     if (s < 0) return;
@@ -465,16 +469,16 @@ bool bkv_prompt_takes(const vkb_context* ctx, const BkvAttn& a) {
     if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_ld % 8 || a.out_ld % 8) return false;
     // A wave of these blocks takes the time of its longest stream whatever the rows; the other kernel's grows with the
     // rows and less with the keys. Microseconds here and there, 8 KV heads of 128, group 4, one stream:
-    //   500 keys, 16 rows 16 and 23; 64 rows 20 and 25          (tables of up to 32 pages: here)
-    //   1000 keys, 32 rows 27 and 25; 64 rows 29 and 34         (64 and 128 tiles of 16 rows, all heads)
-    //   2000 keys, 64 rows 49 and 41; 128 rows 50 and 54        (128 and 256 tiles)
-    //   4000 keys, 128 rows 87 and 73; 256 rows 88 and 115      (256 and 512 tiles)
-    // 8 heads of 64, 1000 keys: 64 tiles 25 and 22, 128 tiles 26 and 29; 20 heads, 2000 keys: 320 tiles 45 and 41.
+    //   500 keys, 16 rows 16 and 20; 64 rows 20 and 20          (tables of up to 32 pages: here)
+    //   1000 keys, 64 rows 29 and 28; 128 rows 30 and 36        (128 and 256 tiles of 16 rows, all heads)
+    //   2000 keys, 64 rows 49 and 31; 128 rows 50 and 45        (128 and 256 tiles)
+    //   4000 keys, 128 rows 87 and 67; 256 rows 87 and 111      (256 and 512 tiles)
+    // 8 heads of 64, 1000 keys: 128 tiles 26 and 23, 256 tiles 26 and 27; 20 heads, 2000 keys: 320 tiles 45 and 39.
     if ((int64_t)a.max_q * a.group < 64) return false;
     if (a.S.ld <= 32) return true;
     const int64_t blocks = most_tiles(a) * a.L.n_kv_head, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
     const int64_t tiles = ((int64_t)a.S.n_tok * a.group + 15) / 16 * a.L.n_kv_head;
-    return tiles >= waves * a.S.ld * (a.d_head == 64 ? 5 : 3) / 2;
+    return tiles >= waves * a.S.ld * (a.d_head == 64 ? 4 : 2);
 }
 
 void run_bkv_prompt(vkb_context* ctx, const BkvAttn& a) {
