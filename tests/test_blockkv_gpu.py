@@ -519,3 +519,48 @@ def test_many_short_streams_beside_long_ones(ctx, d, dtype, most):
     out = cache_of(ctx, plain).attention(0, batch_of(table, start, lens), dev(q), d**-0.5)
     want = plain.attention(table, start, lens, q, d**-0.5)
     assert np.abs(out.cpu().numpy() - want).max() <= TOL[dtype]
+
+
+@pytest.mark.parametrize("dtype,new", [("float32", [1, 2]), ("float16", [200, 150])])
+def test_offsets_above_32_bits(ctx, dtype, new):
+    """Pages at the end of arenas of 2.3 GB: append, attention, read and a page that is copied on a write."""
+    import torch
+    from vokra_b200 import blockkv
+    rng = np.random.default_rng(31)
+    heads, group, d, n_pages = 8, 1, 128, 140000
+    lens = [230, 170]
+    start = np.concatenate([[0], np.cumsum(new)])
+    table, few = tables(rng, lens)
+    plain = filled(rng, few, heads, d)
+    cache = blockkv.BlockKvCache.empty(ctx, 1, heads, d, n_pages)
+    assert cache.k.numel() > 2**31
+    at = n_pages - few
+    for t, a in ((cache.k, plain.k), (cache.v, plain.v), (cache.k_scale, plain.ks), (cache.v_scale, plain.vs)):
+        t[0, at:] = dev(a)
+    high = np.where(table >= 0, table + at, -1).astype(np.int32)
+    b = batch_of(high, start, lens)
+    k, v = (rng.standard_normal((start[-1], heads, d)).astype(dtype) for _ in range(2))
+    q = rng.standard_normal((start[-1], heads * group, d)).astype(dtype)
+    cache.append(0, b, dev(k), dev(v))
+    plain.append(table, start, lens, k, v)
+    for t, a in ((cache.k, plain.k), (cache.v, plain.v), (cache.k_scale, plain.ks), (cache.v_scale, plain.vs)):
+        assert np.array_equal(t[0, at:].cpu().numpy(), a)
+    out = cache.attention(0, b, dev(q), d**-0.5).cpu().numpy()
+    assert np.abs(out - plain.attention(table, start, lens, q, d**-0.5)).max() <= TOL[dtype]
+    got, _ = cache.read(0, b)
+    want, _, _ = plain.rows(table, 1, lens[1])
+    assert np.array_equal(got[start[1]:].cpu().numpy(), want[-new[1]:].astype(np.float32))
+    # stream 0 of a fork keeps its last page, stream 1 writes into a copy; every page in front is taken
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    pages = cache.pages(status)
+    refs = np.ones(n_pages, np.int32)
+    refs[at:] = 0
+    own = high[0, :-(-lens[0] // BLOCK)]
+    refs[own] = 1
+    state = [np.stack([high[0], np.full_like(high[0], -1)]), np.array([lens[0], 0], np.int32), refs]
+    a, c = blockkv.PageState(*map(dev, state)), blockkv.PageState(*map(dev, state))
+    pages.advance(a, c, dev(np.zeros(2, np.int32)), dev(np.array([0, 1], np.int32)))
+    pages.check()
+    copy, last = int(c.table[1, lens[0] // BLOCK]), int(own[lens[0] // BLOCK])
+    assert copy >= at and copy != last
+    assert torch.equal(cache.k[0, copy], cache.k[0, last]) and torch.equal(cache.v_scale[0, copy], cache.v_scale[0, last])

@@ -317,3 +317,24 @@ def test_penalties_that_raise(ctx, dtype, hist, what):
     want, _ = plain_topk(y, k)
     assert np.isin(want[0], kw["history"][0]).any()  # the case is what it says
     check_topk(y, k, ids, lp)
+
+
+def test_offsets_above_32_bits_and_more_rows_than_a_launch(ctx):
+    import torch
+    from vokra_b200 import logits
+    rng = np.random.default_rng(41)
+    rows, vocab, k = 33000, 66001, 3
+    x = torch.zeros(rows, vocab, dtype=torch.float16, device="cuda")
+    assert x.numel() > 2**31
+    some = [0, 32767, 32768, rows - 1]
+    y = rng.standard_normal((len(some), vocab)).astype(np.float16)
+    for r, row in zip(some, y):
+        x[r] = dev(row)
+    history = torch.full((rows, 2), -1, dtype=torch.int32, device="cuda")
+    history[some] = dev(np.stack([np.argsort(-row.astype(np.float32), kind="stable")[:2] for row in y]).astype(np.int32))
+    rules = logits.LogitsRules(history=history, presence=torch.full((rows,), 9.0, device="cuda"))
+    ids, lp = logits.topk(ctx, x, k, rules)
+    want = plain_rules(y, vocab, history=history[some].cpu().numpy(), presence=np.full(len(some), 9, np.float32))
+    check_topk(want, k, ids[some], lp[some])
+    logits.process(ctx, x, rules, out=x)
+    assert np.array_equal(x[some].cpu().numpy(), want.astype(np.float16))
