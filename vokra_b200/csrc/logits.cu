@@ -267,9 +267,10 @@ struct Window {
     }
 };
 
+// (Four blocks an SM: 14.8 us for 128 rows of 51866 in f32; five 17.9 and six 18.6, with spills.)
 template <typename T, int NV>
-__global__ void __launch_bounds__(LG_THREADS) logits_process_kernel(const T* logits, int64_t ld, int vocab,
-                                                                    Rules R, T* out, int64_t out_ld) {
+__global__ void __launch_bounds__(LG_THREADS, 4) logits_process_kernel(const T* logits, int64_t ld, int vocab,
+                                                                       Rules R, T* out, int64_t out_ld) {
     pdl_entry();
     using W = Window<T, NV>;
     extern __shared__ __align__(16) uint32_t lg_cnt[];
@@ -743,8 +744,8 @@ void check_logits(const vkb_context* ctx, const void* logits, int dtype, int64_t
         fail(VKB_ERROR_INVALID_ARGUMENT, "logits: misaligned logits");
 }
 
-// 16-byte vectors of a thread. process, 128 rows of 51866 (f32): 2 vectors 17.2 us, 4 15.6. Selection, 256 rows of
-// 131071 (f16): 2 vectors 108 us, 3 107, 4 104 (fewer looks at a history of 2048 tokens).
+// 16-byte vectors of a thread. process, 128 rows of 51866 (f32): 2 vectors 17.2 us, 4 15.5 (14.8 with four blocks an
+// SM). Selection, 256 rows of 131071 (f16): 2 vectors 108 us, 3 107, 4 104 (fewer looks at a history of 2048 tokens).
 constexpr int NV_F32 = 4, NV_F16 = 2, NV_TOPK = 4;
 constexpr int64_t ROWS_PER_LAUNCH = 32768;  // grid.y
 
