@@ -1,0 +1,124 @@
+"""Attention over the 8-bit cache where blocks, weights or rows of q differ by many powers of two, against 64 bits.
+
+The measure is a row's own: the sum of its weights times the largest |v| of each key that it sees. With 32-bit rows
+a weight is known to 4.4e-5 of itself (2e-4 of values up to 4.5 in test_blockkv_gpu.py); with 16-bit rows it is
+rounded to 2^-11 of itself, the output too, and a score is off by less than 1e-4 for these q: 1.2e-3."""
+import numpy as np
+import pytest
+
+from tests.test_blockkv_gpu import BLOCK, Plain, batch_of, cache_of, dev, filled, tables
+
+pytestmark = pytest.mark.gpu
+
+REL = {"float32": 4.4e-5, "float16": 1.2e-3}
+# rows a stream, query heads of a KV head: tensor-core tiles of 128 rows
+FORMS = [("float16", 90, 2)]
+
+
+def exact(plain, table, start, lens, q, scale):
+    """(out, measure [rows, heads], largest |v| seen [rows, heads]) in 64 bits; a row without keys is 0."""
+    heads, group = plain.k.shape[1], q.shape[1] // plain.k.shape[1]
+    out, size, most = np.zeros(q.shape), np.zeros(q.shape[:2]), np.zeros(q.shape[:2])
+    for s, n in enumerate(lens):
+        k, v, there = plain.rows(table, s, n)
+        nq = start[s + 1] - start[s]
+        for i in range(nq):
+            see = there & (np.arange(n) <= n - nq + i)
+            if not see.any():
+                continue
+            for h in range(q.shape[1]):
+                w = k[see, h // group] @ q[start[s] + i, h].astype(np.float64) * scale
+                w = np.exp(w - w.max())
+                w /= w.sum()
+                vs = v[see, h // group]
+                out[start[s] + i, h] = w @ vs
+                size[start[s] + i, h] = w @ np.abs(vs).max(1)
+                most[start[s] + i, h] = np.abs(vs).max()
+    return out, size, most
+
+
+def run(ctx, plain, table, start, lens, q, scale=0.125, **kw):
+    return cache_of(ctx, plain).attention(0, batch_of(table, start, lens), dev(q), scale=scale, **kw).cpu().numpy()
+
+
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("factor", [2.0**12, 2.0**22, 2.0**60, 2.0**121])
+def test_blocks_that_a_row_does_not_see_do_not_matter(ctx, dtype, new, group, d, factor):
+    """V blocks behind a row's own position, in its tile and its step, have scales far above those that it sees."""
+    rng = np.random.default_rng(d + new + group)
+    heads = 2
+    lens = [67, 160]
+    new = [min(new, n) for n in lens]
+    start = np.concatenate([[0], np.cumsum(new)])
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    plain.vs /= np.float32(64)
+    first = [64, 144]  # positions from here on are in a block with a large scale
+    for s, t in enumerate(first):
+        plain.vs[table[s, t // BLOCK]] = np.float32(factor * 0.02)
+    q = rng.standard_normal((start[-1], heads * group, d)).astype(dtype)
+    got = run(ctx, plain, table, start, lens, q).astype(np.float64)
+    want, size, _ = exact(plain, table, start, lens, q, 0.125)
+    before = np.concatenate([np.arange(n - m, n) < t for n, m, t in zip(lens, new, first)])
+    assert before.any() and not before.all()
+    assert np.isfinite(got[before]).all()
+    assert (np.abs(got - want).max(2)[before] <= REL[dtype] * size[before]).all()
+    if dtype == "float32" and factor < 2.0**100:
+        assert (np.abs(got - want).max(2) <= REL[dtype] * size).all()
+
+
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+def test_an_infinity_in_a_later_token(ctx, dtype, new, group):
+    """Stored as FLT_MAX, it is no business of the rows in front of its block."""
+    rng = np.random.default_rng(5)
+    heads, d, n = 2, 64, 100
+    table, n_pages = tables(rng, [n])
+    plain = Plain(n_pages, heads, d)
+    k, v = (rng.standard_normal((n, heads, d)).astype(dtype) for _ in range(2))
+    v[n - 1, 0, 3] = np.inf
+    v[n - 2, 1, 0] = -np.inf
+    cache = cache_of(ctx, plain)
+    cache.append(0, batch_of(table, [0, n], [n]), dev(k), dev(v))
+    plain.append(table, [0, n], [n], k, v)
+    q = rng.standard_normal((new, heads * group, d)).astype(dtype)
+    got = cache.attention(0, batch_of(table, [0, new], [n]), dev(q), 0.125).cpu().numpy().astype(np.float64)
+    want, size, _ = exact(plain, table, [0, new], [n], q, 0.125)
+    before = np.arange(n - new, n) < 96
+    assert before.any()
+    assert (np.abs(got - want).max(2)[before] <= REL[dtype] * size[before]).all()
+
+
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+@pytest.mark.parametrize("factor", [2.0**10, 2.0**20, 2.0**30])
+def test_large_blocks_of_no_weight(ctx, dtype, new, group, factor):
+    """Blocks with large values and weights near 0 leave the others their bits."""
+    rng = np.random.default_rng(7)
+    heads, d, lens = 2, 64, [300]
+    start = [0, new]
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    big = table[0, :18:2]
+    plain.vs[big] *= np.float32(factor)
+    plain.k[big] = 0
+    plain.k[big, :, :, 0] = -127
+    plain.ks[big] = np.float32(300 / 127)  # scores of these keys are 37 and more below 0: weights of 2^-53
+    q = rng.standard_normal((new, heads * group, d)).astype(dtype)
+    q[..., 0] = 1 + np.abs(q[..., 0])
+    got = run(ctx, plain, table, start, lens, q).astype(np.float64)
+    want, size, _ = exact(plain, table, start, lens, q, 0.125)
+    assert (np.abs(got - want).max(2) <= REL[dtype] * size).all()
+
+
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+def test_blocks_of_scale_zero_have_weight(ctx, dtype, new, group):
+    """Values of 0 whatever the quants, beside small ones: they take their part of the softmax."""
+    rng = np.random.default_rng(8)
+    heads, d, lens = 2, 64, [300]
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    plain.vs[table[0, 1:19:2]] = 0
+    q = rng.standard_normal((new, heads * group, d)).astype(dtype)
+    got = run(ctx, plain, table, [0, new], lens, q).astype(np.float64)
+    want, size, most = exact(plain, table, [0, new], lens, q, 0.125)
+    assert (np.abs(got - want).max(2) <= REL[dtype] * np.maximum(size, most * 0.2)).all()

@@ -19,10 +19,14 @@
 //                     with P (f16) in tensor memory, in S's own columns. It takes
 //                     whichever tile is ready.
 // Scales stay in fp32: a block's K scale multiplies its scores in the exponent's
-// own multiply-add; its V scale, over a running power of two `frame`, is added to
-// the exponent as a logarithm, so a weight comes out scaled at no cost, and the
-// row's sum takes the 16 weights of a block times the inverse. The running
-// maximum (and O) is raised only when a tile exceeds it by 2^8.
+// own multiply-add; its V scale is added to the exponent as a logarithm, so a
+// weight comes out scaled at no cost, and the row's sum takes the 16 weights of
+// a block times the inverse. The running maximum is that of score and logarithm
+// together, over what the row itself sees: a block that it does not see, or whose
+// scaled weights are small, takes no bits from the others. It (and O) is raised
+// only when a half tile exceeds it by 2^8. Scales below 2^-60 count as 2^-60:
+// their values, below 2^-53, are 0 in f16 all the same, and their weights stay
+// above fp32's smallest number in the sum.
 #include "bkv_attn.cuh"
 #include "tc_ptx.cuh"
 
@@ -36,7 +40,7 @@ constexpr int THREADS = 16 * 32;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float L2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2
-constexpr float MIN_W = 9.5367431640625e-7f;  // 2^-20: V scales further below the frame than this count as this
+constexpr float MIN_SCALE = 8.67361738e-19f;  // 2^-60
 constexpr uint32_t POLLS = 1u << 24;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -47,10 +51,8 @@ __device__ __forceinline__ float ex2(float x) {
 
 struct StepScales {
     float k[PAGES];   // K scale * softmax scale * log2(e)
-    float lw[PAGES];  // log2 of the V scale over the frame; -inf: the page is not there
-    float iw[PAGES];  // the inverse of that V scale over the frame; 0 where the page is not there
-    float turn;       // the last step's frame over this one's
-    float frame;
+    float lw[PAGES];  // log2 of the V scale; -inf: the page is not there
+    float iw[PAGES];  // the inverse of the V scale; 0 where the page is not there
     int missing;      // whether a page is not there
 };
 
@@ -178,8 +180,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         }
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_at = at + S_COL + 128 * t, o_at = at + O_COL + D * t;
-        float m = -INFINITY, l = 0.0f;  // running maximum (log2 units), sum
-        float frame = 1.0f;
+        float m = -INFINITY, l = 0.0f;  // running maximum of the scaled weights (log2 units), sum
         for (int i = 0; i < n_half && ok; ++i) {
             const int j = i >> 1, half = i & 1;
             if (!ptx::mbar_wait(&s_full[2 * t + half], j & 1)) { ok = false; break; }
@@ -205,14 +206,13 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 float bm = -INFINITY;
 #pragma unroll
                 for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(x[c]));
-                mx = fmaxf(mx, bm * sc.k[page]);
+                mx = fmaxf(mx, fmaf(bm, sc.k[page], sc.lw[page]));
             }
             const bool raise = mx > m + RAISE;
             const float m_new = raise ? mx : m;
             const float m_use = m_new == -INFINITY ? 0.0f : m_new;
             const float corr = raise ? ex2(m - m_use) : 1.0f;
-            const float corr_o = half ? corr : corr * sc.turn;
-            if (i > 0 && __any_sync(0xffffffffu, corr_o != 1.0f)) {
+            if (i > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
                 // O has to be at rest: the last half's P.V is complete
                 if (!ptx::mbar_wait(&pv_done[2 * t + ((i - 1) & 1)], ((i - 1) >> 1) & 1)) { ok = false; break; }
                 ptx::tc_fence_after();
@@ -222,13 +222,12 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                     ptx::tmem_ld16(o_at + c0, o);
                     ptx::tmem_ld_wait_for(o);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr_o);
+                    for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * corr);
                     ptx::tmem_st16(o_at + c0, o);
                 }
             }
             l *= corr;
             m = m_new;
-            frame = sc.frame;
             // P over S, 64 columns of scores (all in registers by now) becoming 32 of f16 pairs
 #pragma unroll
             for (int c0 = 0; c0 < 2; ++c0) {
@@ -260,7 +259,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         if (ok && n_half > 0 && !ptx::mbar_wait(&pv_done[2 * t + ((n_half - 1) & 1)], ((n_half - 1) >> 1) & 1)) ok = false;
         if (ok) {
             ptx::tc_fence_after();
-            const float fin = frame / l;
+            const float fin = 1.0f / l;
             __half* to = reinterpret_cast<__half*>(A.out) + (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D;
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -317,7 +316,6 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         int ids = ids_of(0), ids_next = ids_of(1);
         load(ids);
         if (warp == 8) load_scales(ids);
-        float frame = __uint_as_float(0x00800000u);
         uint64_t *empty = is_v ? v_empty : k_empty, *full = is_v ? v_full : k_full;
         for (int j = 0; j < n_steps && ok; ++j) {
             const int st = j & 1;
@@ -352,25 +350,15 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             if (warp == 8) {
                 // (scales[j & 3] was last read for step j - 4, which ended before K's buffer of step j - 2 came free)
                 StepScales& sc = scales[j & 3];
-                float vmax = vs;
-#pragma unroll
-                for (int o = 4; o > 0; o >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-                const float pow2 = fmaxf(frame, __uint_as_float(__float_as_uint(vmax) & 0x7f800000u));
-                const float inv = __uint_as_float(0x7f000000u - __float_as_uint(pow2));
                 const unsigned there = __ballot_sync(0xffffffffu, ids >= 0);
                 if (lane < PAGES) {
-                    const float w = fmaxf(vs * inv, MIN_W);
+                    const float w = fmaxf(vs, MIN_SCALE);
                     sc.k[lane] = fmaxf(ks * (A.scale * L2E), 1e-37f);  // above 0: a masked -inf stays -inf
                     sc.lw[lane] = ids >= 0 ? log2f(w) : -INFINITY;
                     sc.iw[lane] = ids >= 0 ? 1.0f / w : 0.0f;
                 }
                 const int valid = min(PAGES, n_pages - j * PAGES);
-                if (lane == 0) {
-                    sc.turn = j ? frame * inv : 1.0f;
-                    sc.frame = pow2;
-                    sc.missing = (there & ((1u << valid) - 1)) != (1u << valid) - 1;
-                }
-                frame = __shfl_sync(0xffffffffu, pow2, 0);
+                if (lane == 0) sc.missing = (there & ((1u << valid) - 1)) != (1u << valid) - 1;
                 __syncwarp();
             }
             ptx::fence_proxy_async_smem();
