@@ -11,8 +11,8 @@ from tests.test_blockkv_gpu import BLOCK, Plain, batch_of, cache_of, dev, filled
 pytestmark = pytest.mark.gpu
 
 REL = {"float32": 4.4e-5, "float16": 1.2e-3}
-# rows a stream, query heads of a KV head: tensor-core tiles of 128 rows
-FORMS = [("float16", 90, 2)]
+# rows a stream, query heads of a KV head: 8 rows of a tile, 16 rows of a tile, tensor-core tiles of 128 rows
+FORMS = [("float32", 6, 1), ("float32", 40, 2), ("float16", 6, 1), ("float16", 6, 4), ("float16", 90, 2)]
 
 
 def exact(plain, table, start, lens, q, scale):

@@ -18,8 +18,10 @@
 //  - V is stored channel by channel, so 16 bytes of (page c, channel 8i + g) are
 //    the 16 tokens whose weights the lane holds: four k steps of P.V (m16n8k16).
 //    int8 -> f16 is exact (a byte permute into 1024 + u, minus 1152). The V scale
-//    multiplies the weights in fp32; weights enter divided by a running power of
-//    two above the V scales, so that f16 holds them whatever the scale.
+//    multiplies the weights in fp32; they enter divided by the row's `frame`, a
+//    power of two near the row's largest product of weight and V scale so far, so
+//    that f16 holds what counts whatever the scales. It falls with the weights when
+//    the row's maximum rises, and blocks that the row does not see are no part of it.
 //
 // Tiles of 8 query rows (SPLIT) hold p1 in rows 0..7 of the 16-row operand and
 // p2 in rows 8..15, likewise the high and low f16 parts of the weights: 2^-21
@@ -36,6 +38,7 @@
 #include "bkv_attn.cuh"
 #include "tc_ptx.cuh"
 #include <algorithm>
+#include <cfloat>
 
 namespace vkb {
 namespace {
@@ -528,11 +531,12 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
 
             float m[NR], l[NR];
             float o[NT][4];
-            float frame = __uint_as_float(0x00800000u);  // power of two at or above half of every V scale so far
+            float frame[NR];  // O is in units of it
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 m[i] = -INFINITY;
                 l[i] = 0.0f;
+                frame[i] = FLT_MIN;
             }
 #pragma unroll
             for (int i = 0; i < NT; ++i)
@@ -601,23 +605,12 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
 
                 // ---- softmax step. Lane c holds tokens 0..15 of page 4 ch + c: x[row][token]
                 const int key0 = 64 * ch + 16 * c;
-                float w_scale;
+                float w_scale[NR];
                 float corr_o[NR];
                 float x[NR][16];
-                {
-                    // the V scales' frame
-                    float vmax = fmaxf(vs, __shfl_xor_sync(0xffffffffu, vs, 1));
-                    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-                    const float pow2 = fmaxf(frame, __uint_as_float(__float_as_uint(vmax) & 0x7f800000u));
-                    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(pow2));
-                    w_scale = vs * inv;
-#pragma unroll
-                    for (int i = 0; i < NR; ++i) corr_o[i] = frame * inv;
-                    frame = pow2;
-                }
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
-                        float f = ks * row_fac[i];
+                    float f = ks * row_fac[i];
                     if (f < 1e-37f) f = 1e-37f;  // above 0: a masked token's -inf stays -inf (and NaN stays NaN)
                     float mx = -INFINITY;
 #pragma unroll
@@ -640,6 +633,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
 #pragma unroll
                     for (int t = 0; t < 16; ++t) mx = fmaxf(mx, x[i][t]);
                     mx *= f;
+                    const float mine_max = mx;  // of the lane's page
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
                     const float m_new = fmaxf(m[i], mx);
@@ -653,7 +647,14 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                         sum += x[i][t];
                     }
                     l[i] = fmaf(l[i], corr, sum);
-                    corr_o[i] *= corr;
+                    float w_max = ex2(mine_max - m_use) * vs;
+                    w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, 1));
+                    w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, 2));
+                    const float old = frame[i] * corr;
+                    frame[i] = __uint_as_float(__float_as_uint(fmaxf(fmaxf(old, w_max), FLT_MIN)) & 0x7f800000u);
+                    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(frame[i]));
+                    corr_o[i] = old * inv;
+                    w_scale[i] = fminf(vs * inv, FLT_MAX);  // (finite: a hidden page's weights are 0 times this)
                 }
                 bool turn = corr_o[0] != 1.0f;
                 if constexpr (NR == 2) turn |= corr_o[1] != 1.0f;
@@ -672,8 +673,8 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 for (int t = 0; t < 4; ++t) {
 #pragma unroll
                     for (int i = 0; i < NR; ++i) {
-                        const float y0 = x[i][4 * t] * w_scale, y1 = x[i][4 * t + 1] * w_scale, y2 = x[i][4 * t + 2] * w_scale,
-                                    y3 = x[i][4 * t + 3] * w_scale;
+                        const float y0 = x[i][4 * t] * w_scale[i], y1 = x[i][4 * t + 1] * w_scale[i], y2 = x[i][4 * t + 2] * w_scale[i],
+                                    y3 = x[i][4 * t + 3] * w_scale[i];
                         const uint32_t h0 = pack_f16(y0, y1), h1 = pack_f16(y2, y3);
                         if constexpr (SPLIT) {
                             pa[t][0] = h0;
@@ -733,7 +734,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 const int r = tile * TR + i * 8 + g;
                 const int tok = r / A.group, head = h * A.group + r % A.group;
                 if (tok >= n_q) continue;
-                const float fin = alone ? (l[i] == 0.0f ? 0.0f : frame / l[i]) : frame;
+                const float fin = alone ? (l[i] == 0.0f ? 0.0f : frame[i] / l[i]) : frame[i];
                 const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
                 float* po = A.warp_o + (part * TR + i * 8 + g) * D + 2 * c;
                 if (!alone && c == 0) A.warp_ml[part * TR + i * 8 + g] = make_float2(m[i], l[i]);
