@@ -122,3 +122,27 @@ def test_blocks_of_scale_zero_have_weight(ctx, dtype, new, group):
     got = run(ctx, plain, table, [0, new], lens, q).astype(np.float64)
     want, size, most = exact(plain, table, [0, new], lens, q, 0.125)
     assert (np.abs(got - want).max(2) <= REL[dtype] * np.maximum(size, most * 0.2)).all()
+
+
+@pytest.mark.parametrize("dtype,new,group,n", [("float32", 1, 1, 40000), ("float16", 1, 1, 40000), ("float16", 3, 4, 40000), ("float16", 90, 1, 470)])
+def test_many_small_weights(ctx, dtype, new, group, n):
+    """One key of weight 1 and value 0, the others of weight 2^-26 and value 100 each."""
+    rng = np.random.default_rng(9)
+    heads, d = 1, 64
+    table, n_pages = tables(rng, [n])
+    plain = Plain(n_pages, heads, d)
+    plain.k[..., 0] = -127
+    plain.k[table[0, 0], :, 0, 0] = 127
+    plain.ks[:] = np.float32(26 * np.log(2) / 254)
+    plain.v[:] = 127
+    plain.v[table[0, 0], :, :, 0] = 0
+    plain.vs[:] = np.float32(100 / 127)
+    q = np.zeros((new, heads * group, d), dtype)
+    q[..., 0] = 1
+    got = run(ctx, plain, table, [0, new], [n], q, scale=1.0).astype(np.float64)
+    # every row sees the first key and n - new + 1 or more others
+    others = n - new + np.arange(new)
+    w = 2.0**-26 * others
+    want = (100 * w / (1 + w))[:, None, None]
+    # the smallest step of f16 is 6e-8; equal weights are rounded alike: 2^-11, and the output 2^-11
+    assert (np.abs(got - want) <= REL[dtype] * want + (3e-8 if dtype == "float16" else 0)).all()

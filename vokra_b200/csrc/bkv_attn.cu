@@ -20,7 +20,8 @@
 //    int8 -> f16 is exact (a byte permute into 1024 + u, minus 1152). The V scale
 //    multiplies the weights in fp32; they enter divided by the row's `frame`, a
 //    power of two near the row's largest product of weight and V scale so far, so
-//    that f16 holds what counts whatever the scales. It falls with the weights when
+//    that f16 holds what counts whatever the scales, and times 2^14, so that a
+//    weight keeps its bits down to 2^-28 of the row's largest. The frame falls with the weights when
 //    the row's maximum rises, and blocks that the row does not see are no part of it.
 //
 // Tiles of 8 query rows (SPLIT) hold p1 in rows 0..7 of the 16-row operand and
@@ -44,6 +45,8 @@ namespace vkb {
 namespace {
 
 constexpr int BKV_SEQ_PER_LAUNCH = 512;
+constexpr float W_UP = 16384.0f;  // weights over the frame are below 2, their f16 forms below 2^15
+constexpr float MIN_FRAME = FLT_MIN * W_UP;
 constexpr float L2E = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -531,12 +534,12 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
 
             float m[NR], l[NR];
             float o[NT][4];
-            float frame[NR];  // O is in units of it
+            float frame[NR];  // O is in units of frame / W_UP
 #pragma unroll
             for (int i = 0; i < NR; ++i) {
                 m[i] = -INFINITY;
                 l[i] = 0.0f;
-                frame[i] = FLT_MIN;
+                frame[i] = MIN_FRAME;
             }
 #pragma unroll
             for (int i = 0; i < NT; ++i)
@@ -651,10 +654,10 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                     w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, 1));
                     w_max = fmaxf(w_max, __shfl_xor_sync(0xffffffffu, w_max, 2));
                     const float old = frame[i] * corr;
-                    frame[i] = __uint_as_float(__float_as_uint(fmaxf(fmaxf(old, w_max), FLT_MIN)) & 0x7f800000u);
+                    frame[i] = __uint_as_float(__float_as_uint(fmaxf(fmaxf(old, w_max), MIN_FRAME)) & 0x7f800000u);
                     const float inv = __uint_as_float(0x7f000000u - __float_as_uint(frame[i]));
                     corr_o[i] = old * inv;
-                    w_scale[i] = fminf(vs * inv, FLT_MAX);  // (finite: a hidden page's weights are 0 times this)
+                    w_scale[i] = fminf(vs * inv * W_UP, FLT_MAX);  // (finite: a hidden page's weights are 0 times this)
                 }
                 bool turn = corr_o[0] != 1.0f;
                 if constexpr (NR == 2) turn |= corr_o[1] != 1.0f;
@@ -734,7 +737,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 const int r = tile * TR + i * 8 + g;
                 const int tok = r / A.group, head = h * A.group + r % A.group;
                 if (tok >= n_q) continue;
-                const float fin = alone ? (l[i] == 0.0f ? 0.0f : frame[i] / l[i]) : frame[i];
+                const float unit = frame[i] * (1.0f / W_UP), fin = alone ? (l[i] == 0.0f ? 0.0f : unit / l[i]) : unit;
                 const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
                 float* po = A.warp_o + (part * TR + i * 8 + g) * D + 2 * c;
                 if (!alone && c == 0) A.warp_ml[part * TR + i * 8 + g] = make_float2(m[i], l[i]);

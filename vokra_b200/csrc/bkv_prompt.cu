@@ -40,6 +40,7 @@ constexpr int THREADS = 16 * 32;
 constexpr uint32_t TMEM_COLS = 512;
 constexpr float L2E = 1.4426950408889634f;
 constexpr float RAISE = 8.0f;       // log2
+constexpr float UP = 7.0f;          // log2: weights enter f16 times 2^7, below 2^15, and keep their bits down to 2^-21 of the maximum
 constexpr float MIN_SCALE = 8.67361738e-19f;  // 2^-60
 constexpr uint32_t POLLS = 1u << 24;
 
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
         }
         const uint32_t at = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t s_at = at + S_COL + 128 * t, o_at = at + O_COL + D * t;
-        float m = -INFINITY, l = 0.0f;  // running maximum of the scaled weights (log2 units), sum
+        float m = -INFINITY, l = 0.0f;  // running maximum of the scaled weights less UP (log2 units), sum
         for (int i = 0; i < n_half && ok; ++i) {
             const int j = i >> 1, half = i & 1;
             if (!ptx::mbar_wait(&s_full[2 * t + half], j & 1)) { ok = false; break; }
@@ -208,8 +209,8 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
                 for (int c = 0; c < 16; ++c) bm = fmaxf(bm, __uint_as_float(x[c]));
                 mx = fmaxf(mx, fmaf(bm, sc.k[page], sc.lw[page]));
             }
-            const bool raise = mx > m + RAISE;
-            const float m_new = raise ? mx : m;
+            const bool raise = mx > m + (RAISE + UP);
+            const float m_new = raise ? mx - UP : m;
             const float m_use = m_new == -INFINITY ? 0.0f : m_new;
             const float corr = raise ? ex2(m - m_use) : 1.0f;
             if (i > 0 && __any_sync(0xffffffffu, corr != 1.0f)) {
