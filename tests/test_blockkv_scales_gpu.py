@@ -146,3 +146,18 @@ def test_many_small_weights(ctx, dtype, new, group, n):
     want = (100 * w / (1 + w))[:, None, None]
     # the smallest step of f16 is 6e-8; equal weights are rounded alike: 2^-11, and the output 2^-11
     assert (np.abs(got - want) <= REL[dtype] * want + (3e-8 if dtype == "float16" else 0)).all()
+
+
+@pytest.mark.parametrize("n", [64, 65, 700, 5000])
+def test_the_largest_values(ctx, n):
+    """Values near the largest finite number: their average is finite, however the keys are shared out."""
+    rng = np.random.default_rng(10)
+    heads, d = 2, 64
+    table, n_pages = tables(rng, [n])
+    plain = filled(rng, n_pages, heads, d)
+    plain.vs[:] = np.float32(np.finfo(np.float32).max / 130)
+    q = rng.standard_normal((2, heads * 2, d)).astype(np.float32)
+    got = run(ctx, plain, table, [0, 2], [n], q).astype(np.float64)
+    want, size, _ = exact(plain, table, [0, 2], [n], q, 0.125)
+    assert np.isfinite(got).all()
+    assert (np.abs(got - want).max(2) <= REL["float32"] * size).all()

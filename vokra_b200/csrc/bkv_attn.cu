@@ -105,7 +105,7 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
 struct AttnArgs : BkvAttn {
     int q_vec, out_vec;
     float* warp_o;    // [blocks * AW][2][rows][D]: a warp's parts of items that it shares with others
-    float2* warp_ml;  // [blocks * AW][2][rows]
+    float2* warp_ml;  // [blocks * AW][2][rows]: their maximum and sum; the part's rows are divided by that sum
     float* block_o;   // [blocks][2][rows][D]: the same of a block
     float2* block_ml;
     unsigned* arrived;  // [blocks], 0 at rest: blocks that have left their part of the item that starts in block i
@@ -271,10 +271,11 @@ __device__ __forceinline__ void store_pair(const AttnArgs& A, int64_t at, float 
 }
 
 // Joins rows r and (if it is not negative) r2 of `n` parts, in order, a warp for both at once: their loads are one round
-// trip. Part i's rows are o(i) and their (max, sum) ml(i). To the output, or (to_o) to another part.
+// trip. Part i's rows are o(i) and their (max, sum) ml(i). To the output, or (to_o) to another part. The parts are averages,
+// and `share`, a power of two at or below 1 / keys, keeps their sum one: it holds whatever fp32 values V has.
 template <int D, class FO, class FM>
-__device__ __forceinline__ void join_rows(const AttnArgs& A, int n, int r, int r2, int64_t row_at, int tile_row0, int h, FO o,
-                                          FM ml, float* to_o, float2* to_ml) {
+__device__ __forceinline__ void join_rows(const AttnArgs& A, int n, int r, int r2, int64_t row_at, int tile_row0, int h, float share,
+                                          FO o, FM ml, float* to_o, float2* to_ml) {
     const int lane = threadIdx.x & 31;
     constexpr int C = D / 32;  // channels of a lane, as pairs 64 apart (one alone for D = 32, three for D = 96)
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, y[2][C];
@@ -316,9 +317,10 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, int n, int r, int r
                 const float m_new = fmaxf(m[k], x[k][p].x);
                 const float m_use = m_new == -INFINITY ? 0.0f : m_new;
                 const float a = ex2(m[k] - m_use), b = ex2(x[k][p].x - m_use);
-                l[k] = l[k] * a + x[k][p].y * b;
+                const float lb = x[k][p].y * b, part = lb * share;
+                l[k] = l[k] * a + lb;
 #pragma unroll
-                for (int i = 0; i < C; ++i) y[k][i] = y[k][i] * a + v[k][p][i] * b;
+                for (int i = 0; i < C; ++i) y[k][i] = y[k][i] * a + v[k][p][i] * part;
                 m[k] = m_new;
             }
     }
@@ -326,13 +328,13 @@ __device__ __forceinline__ void join_rows(const AttnArgs& A, int n, int r, int r
     for (int k = 0; k < 2; ++k) {
         const int rk = k ? r2 : r;
         if (rk < 0) continue;
+        const float inv = l[k] == 0.0f ? 0.0f : 1.0f / (l[k] * share);
         if (to_o) {
 #pragma unroll
-            for (int i = 0; i < C; ++i) to_o[rk * D + ch(i)] = y[k][i];
+            for (int i = 0; i < C; ++i) to_o[rk * D + ch(i)] = y[k][i] * inv;
             if (lane == 0) to_ml[rk] = make_float2(m[k], l[k]);
         } else {
             const int row = tile_row0 + rk, tok = row / A.group, head = h * A.group + row % A.group;
-            const float inv = l[k] == 0.0f ? 0.0f : 1.0f / l[k];
             const int64_t at = (row_at + tok) * A.out_ld + (int64_t)head * D;
 #pragma unroll
             for (int i = 0; i < C; i += C % 2 ? 1 : 2) {
@@ -737,7 +739,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 const int r = tile * TR + i * 8 + g;
                 const int tok = r / A.group, head = h * A.group + r % A.group;
                 if (tok >= n_q) continue;
-                const float unit = frame[i] * (1.0f / W_UP), fin = alone ? (l[i] == 0.0f ? 0.0f : unit / l[i]) : unit;
+                const float fin = l[i] == 0.0f ? 0.0f : frame[i] * (1.0f / W_UP) / l[i];
                 const int64_t at = (int64_t)(first_row + tok) * A.out_ld + (int64_t)head * D + 2 * c;
                 float* po = A.warp_o + (part * TR + i * 8 + g) * D + 2 * c;
                 if (!alone && c == 0) A.warp_ml[part * TR + i * 8 + g] = make_float2(m[i], l[i]);
@@ -765,6 +767,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
     if (!ok && lane == 0) atomicExch(A.err, 1);
     __syncthreads();
 
+    auto share_of = [&](int s) { return __uint_as_float((uint32_t)(95 + __clz(max(st.keys[s], 1))) << 23); };  // 2^-bits(keys)
     // ---- parts of one item within the block, then what the block shares with others
     // lane i: whether part i is the block's first one of its item (the second part of a warp starts its item)
     const unsigned heads = __ballot_sync(
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
             auto nth = [&](int j) { return ((int64_t)blockIdx.x * AW * 2 + (j ? 2 * (i / 2 + j) : i)) * TR; };
             while (job < rows) {
                 const int second = job + AW < rows ? job + AW : -1;
-                join_rows<D>(A, n, job, second, st.first[p.s], p.tile * TR, p.h, [&](int j) { return A.warp_o + nth(j) * D; },
+                join_rows<D>(A, n, job, second, st.first[p.s], p.tile * TR, p.h, share_of(p.s), [&](int j) { return A.warp_o + nth(j) * D; },
                             [&](int j) { return A.warp_ml + nth(j); }, whole ? nullptr : A.block_o + to * D,
                             whole ? nullptr : A.block_ml + to);
                 job += second < 0 ? AW : 2 * AW;
@@ -816,7 +819,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
         // the item starts somewhere in its first block's range, and at the start of every other one's
         auto nth = [&](int b) { return ((first + b) * 2 + (b == 0 && p.u0 != first * total / n_block ? 1 : 0)) * TR; };
         for (int r = warp; r < rows; r += 2 * AW)
-            join_rows<D>(A, n, r, r + AW < rows ? r + AW : -1, st.first[p.s], p.tile * TR, p.h, [&](int b) { return A.block_o + nth(b) * D; },
+            join_rows<D>(A, n, r, r + AW < rows ? r + AW : -1, st.first[p.s], p.tile * TR, p.h, share_of(p.s), [&](int b) { return A.block_o + nth(b) * D; },
                         [&](int b) { return A.block_ml + nth(b); }, nullptr, nullptr);
     }
 }
