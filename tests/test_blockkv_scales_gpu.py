@@ -161,3 +161,32 @@ def test_the_largest_values(ctx, n):
     want, size, _ = exact(plain, table, [0, 2], [n], q, 0.125)
     assert np.isfinite(got).all()
     assert (np.abs(got - want).max(2) <= REL["float32"] * size).all()
+
+
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_with_an_infinity(ctx, dtype, new, group, d):
+    """NaN, whatever the signs of the few keys that the row sees; a row without any key is 0, whatever it holds."""
+    rng = np.random.default_rng(11)
+    heads = 2
+    lens, rows = [new, new - 3], [new, new]
+    start = np.array([0, new, 2 * new])
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    plain.k[table[:, 0], :, 0] = -np.abs(plain.k[table[:, 0], :, 0]) - (plain.k[table[:, 0], :, 0] == 0)
+    cache = cache_of(ctx, plain)
+    b = batch_of(table, start, lens)
+    q = rng.standard_normal((2 * new, heads * group, d)).astype(dtype)
+    clean = cache.attention(0, b, dev(q), 0.125).cpu().numpy()
+    bad = np.zeros(q.shape[:2], bool)
+    none = np.zeros(q.shape[:2], bool)
+    for r, h, x in ((0, 0, np.inf), (0, 1, -np.inf), (1, 0, np.inf), (new + 3, 1, np.inf), (new + 4, 0, np.nan)):
+        q[r, h, 5] = x
+        bad[r, h] = True
+    for r, h, x in ((new, 0, np.inf), (new + 1, 1, np.nan), (new + 2, 0, -np.inf)):
+        q[r, h, 7] = x
+        none[r, h] = True
+    got = cache.attention(0, b, dev(q), 0.125).cpu().numpy()
+    assert np.isnan(got[bad]).all()
+    assert (got[new:new + 3] == 0).all()
+    assert np.array_equal(got[~(bad | none)], clean[~(bad | none)])

@@ -513,9 +513,10 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 // planes: q = amax / 127 * (p1 + p2 / 254 + p3 / 254^2). Two of them hold it to 2^-16 of the row's
                 // largest, three to 2^-24. Below 1e-35 a row's products with any scale count as zero.
                 const float unit = amax > 1e-35f ? 127.0f / amax : 0.0f;
-                row_fac[half_row] = number && amax < INFINITY ? amax * (1.0f / (127.0f * (P3 ? 64516.0f : 254.0f))) * (A.scale * L2E)
-                                                              : __uint_as_float(0x7fc00000u);
                 limit[half_row] = real ? max(0, min(n_keys, n_keys - n_q + tok + 1)) : 0;
+                row_fac[half_row] = amax * (1.0f / (127.0f * (P3 ? 64516.0f : 254.0f))) * (A.scale * L2E);
+                // NaN where q has an infinity or NaN; a row in front of the first key is 0, whatever it holds
+                if (!(number && amax < INFINITY)) row_fac[half_row] = limit[half_row] > 0 ? __uint_as_float(0x7fc00000u) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < KW; ++i) {
                     float y[4];
