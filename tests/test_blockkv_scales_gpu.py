@@ -190,3 +190,20 @@ def test_rows_with_an_infinity(ctx, dtype, new, group, d):
     assert np.isnan(got[bad]).all()
     assert (got[new:new + 3] == 0).all()
     assert np.array_equal(got[~(bad | none)], clean[~(bad | none)])
+
+
+@pytest.mark.parametrize("size", [1e-33, 1e-36, 1e-39])
+@pytest.mark.parametrize("d", [64, 96])
+def test_rows_of_tiny_values(ctx, size, d):
+    """Small rows of q over keys as large as they are small: scores of ordinary size. A q below 1.2e-38 has fewer bits
+    itself (steps of 1.4e-45, exact in the plain form too)."""
+    rng = np.random.default_rng(12)
+    heads, lens = 2, [200]
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    up = min(1 / size, 1e37)
+    plain.ks *= np.float32(up)
+    q = (rng.standard_normal((5, heads * 2, d)) * size).astype(np.float32)
+    got = run(ctx, plain, table, [0, 5], lens, q, scale=0.125 / (size * up)).astype(np.float64)
+    want, size_of, _ = exact(plain, table, [0, 5], lens, q, np.float64(np.float32(0.125 / (size * up))))
+    assert (np.abs(got - want).max(2) <= REL["float32"] * size_of).all()

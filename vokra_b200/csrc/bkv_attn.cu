@@ -448,6 +448,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
             uint32_t qa[KW / 2][4];
             uint32_t qb[KW / 2][SPLIT ? 2 : 4];  // the third plane (SPLIT, 32-bit rows), or the second one of 16 rows
             float row_fac[NR];  // multiplies a score: scale * log2(e) * the units of the planes
+            float row_down = 1.0f;  // so does this (a row of 32 bits: a tile has one a lane)
             int limit[NR];      // keys that the row sees
             if (c0 < c_last)
 #pragma unroll
@@ -510,9 +511,21 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 number = (__ballot_sync(0xffffffffu, number) >> (4 * g) & 15) == 15;
+                // Small rows (of 32 bits) are taken times 2^64: their scores need not be small, for K reaches FLT_MAX.
+                if constexpr (P3) {
+                    const bool small = amax < 0x1p-60f;
+                    row_down = small ? 0x1p-64f : 1.0f;
+                    if (small) {
+                        amax *= 0x1p64f;
+#pragma unroll
+                        for (int i = 0; i < KW; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[i][e] *= 0x1p64f;
+                    }
+                }
                 // planes: q = amax / 127 * (p1 + p2 / 254 + p3 / 254^2). Two of them hold it to 2^-16 of the row's
-                // largest, three to 2^-24. Below 1e-35 a row's products with any scale count as zero.
-                const float unit = amax > 1e-35f ? 127.0f / amax : 0.0f;
+                // largest, three to 2^-24.
+                const float unit = amax > 0.0f ? 127.0f / amax : 0.0f;
                 limit[half_row] = real ? max(0, min(n_keys, n_keys - n_q + tok + 1)) : 0;
                 row_fac[half_row] = amax * (1.0f / (127.0f * (P3 ? 64516.0f : 254.0f))) * (A.scale * L2E);
                 // NaN where q has an infinity or NaN; a row in front of the first key is 0, whatever it holds
@@ -617,6 +630,7 @@ __global__ void __launch_bounds__(32 * Ring<D>::AW, 1) bkv_attn_kernel(AttnArgs 
 #pragma unroll
                 for (int i = 0; i < NR; ++i) {
                     float f = ks * row_fac[i];
+                    if constexpr (P3) f *= row_down;
                     if (f < 1e-37f) f = 1e-37f;  // above 0: a masked token's -inf stays -inf (and NaN stays NaN)
                     float mx = -INFINITY;
 #pragma unroll
