@@ -124,6 +124,9 @@ VKB_API vkb_status vkb_context_set_precision(vkb_context* ctx, int precision);
 VKB_API uint64_t vkb_context_launch_count(const vkb_context* ctx);
 /* Bytes of device scratch the context holds for calls that size their own
  * workspace (it only grows); vkb_attention_dense_noalloc never touches it.
+ * A workspace whose address is in a recorded graph stays allocated, beside the
+ * larger one that later calls use, until the context is destroyed; replay such
+ * graphs before that, and on one stream with the context's other calls.
  * No counterpart in the reference (a diagnostics accessor). */
 VKB_API size_t vkb_context_workspace_bytes(const vkb_context* ctx);
 

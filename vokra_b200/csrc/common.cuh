@@ -97,6 +97,27 @@ struct DevBuf {
     template <class T> T* as() const { return reinterpret_cast<T*>(p); }
 };
 
+// A buffer that grows when a call needs more. One whose address went into a
+// graph that was being recorded is kept until the context ends: the graph may be
+// replayed at any time. (The others are freed, so repeated growth holds nothing.)
+struct Scratch : DevBuf {
+    std::vector<DevBuf> kept;
+    bool recorded = false;
+    void ensure(size_t bytes, cudaStream_t stream) {
+        if (n < bytes) {
+            VKB_CUDA(cudaStreamSynchronize(stream));
+            if (recorded) kept.push_back(std::move(static_cast<DevBuf&>(*this)));
+            recorded = false;
+            alloc(bytes);
+        }
+        if (!recorded) {
+            cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+            if (cudaStreamIsCapturing(stream, &status) != cudaSuccess) cudaGetLastError();  // (the launch will say what is wrong)
+            recorded = status == cudaStreamCaptureStatusActive;
+        }
+    }
+};
+
 }  // namespace vkb
 
 // The context: one per GPU. Owns a stream and a grow-at-setup workspace that
@@ -108,22 +129,17 @@ struct vkb_context {
     cudaStream_t stream = nullptr;
     uint64_t launches = 0;
     int precision = VKB_PREC_SPLIT;  // tensor-core operand precision (vkb_context_set_precision)
-    vkb::DevBuf workspace;
+    vkb::Scratch workspace;
     vkb::DevBuf err_flag;  // int set by a kernel whose bounded wait gave up
     vkb::DevBuf tile_ctr;  // per-tile arrival counters of in-kernel split-K reductions (each returns to 0)
     vkb::DevBuf frontend;  // log-mel tables (window, twiddles, mel bank) + per-clip maxima
     int frontend_mels = 0; // mel count the tables were built for
-    vkb::DevBuf wplane;    // f16 weight plane of the SS encoder GEMM (n_pad x k halves, grown on first use)
+    vkb::Scratch wplane;   // f16 weight plane of the SS encoder GEMM (n_pad x k halves, grown on first use)
     // Programmatic dependent launch: each kernel may start while the previous
     // one in the stream drains; it waits (griddepcontrol.wait) before touching
     // anything that kernel wrote (VKB_PDL=0 turns it off).
     bool pdl = true;
-    void ensure_workspace(size_t bytes) {
-        if (workspace.n < bytes) {
-            VKB_CUDA(cudaStreamSynchronize(stream));
-            workspace.alloc(bytes);
-        }
-    }
+    void ensure_workspace(size_t bytes) { workspace.ensure(bytes, stream); }
     void count(int n = 1) { launches += (uint64_t)n; }
 };
 

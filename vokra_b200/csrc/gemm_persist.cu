@@ -672,10 +672,7 @@ template <int FMT, int EG>
 static void launch_pair(vkb_context* ctx, const vkb_weight* w, int64_t m, const __half* a16, const PEpi& e, int* err) {
     using C = PairCfg<EG>;
     const size_t bytes = (size_t)w->n_pad * w->k * sizeof(__half);
-    if (ctx->wplane.n < bytes) {
-        VKB_CUDA(cudaStreamSynchronize(ctx->stream));
-        ctx->wplane.alloc(bytes);
-    }
+    ctx->wplane.ensure(bytes, ctx->stream);
     launch_pdl(ctx, dequant_plane_kernel<FMT>, dim3((unsigned)(w->k / STAGE_K), (unsigned)(w->n_pad / TILE_N)), TILE_N, 0,
                w->qs.as<uint8_t>(), w->sc.as<uint8_t>(), w->k, ctx->wplane.as<__half>());
     VKB_CUDA(cudaGetLastError());
@@ -719,10 +716,7 @@ static void launch_persist(vkb_context* ctx, const vkb_weight* w, int64_t m, con
     const int n_tiles = (int)(w->n_pad / TILE_N);
     if (SS) {
         const size_t bytes = (size_t)w->n_pad * w->k * sizeof(__half);
-        if (ctx->wplane.n < bytes) {
-            VKB_CUDA(cudaStreamSynchronize(ctx->stream));
-            ctx->wplane.alloc(bytes);
-        }
+        ctx->wplane.ensure(bytes, ctx->stream);
         launch_pdl(ctx, dequant_plane_kernel<FMT>, dim3((unsigned)(w->k / STAGE_K), (unsigned)n_tiles), TILE_N, 0,
                    w->qs.as<uint8_t>(), w->sc.as<uint8_t>(), w->k, ctx->wplane.as<__half>());
         VKB_CUDA(cudaGetLastError());
