@@ -116,6 +116,10 @@ VKB_API vkb_status vkb_context_destroy(vkb_context* ctx);
  * same device, or cudaStreamLegacy = (void*)0x1 for the legacy default stream;
  * NULL = the context's own stream). */
 VKB_API vkb_status vkb_context_set_stream(vkb_context* ctx, void* stream);
+/* Waits for the context's stream. VKB_ERROR_OTHER where a wait inside a kernel
+ * launched since the last call gave up (every wait is bounded): some result of
+ * those calls is not complete. The report is given once, and the context stays
+ * usable. Device-pointer calls are asynchronous and cannot report it themselves. */
 VKB_API vkb_status vkb_context_synchronize(vkb_context* ctx);
 /* Selects the tensor-core operand precision (vkb_precision). */
 VKB_API vkb_status vkb_context_set_precision(vkb_context* ctx, int precision);
@@ -137,6 +141,9 @@ VKB_API size_t vkb_context_workspace_bytes(const vkb_context* ctx);
  * and returns; the call then reports VKB_ERROR_OTHER and clears the flag, and
  * the context remains usable. No GPU fault, trap or hang is involved. */
 VKB_API vkb_status vkb_context_selftest_bounded_wait(vkb_context* ctx, uint32_t polls);
+/* The same kernel as a device-pointer call would launch it: returns at once, and
+ * vkb_context_synchronize reports the wait that gave up. */
+VKB_API vkb_status vkb_context_selftest_stalled_kernel(vkb_context* ctx, uint32_t polls);
 
 /* ---- quantized Linear: Compute::gemm_q_f32 (compute.rs:943) ---------------- */
 

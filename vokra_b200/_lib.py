@@ -150,6 +150,7 @@ SIGNATURES = {
     "vkb_gguf_inspect": (C.c_int, [P, SZ, P, P]),
     "vkb_kv_copy_stream": (C.c_int, [P, I32, I32, I32]),
     "vkb_context_selftest_bounded_wait": (C.c_int, [P, U32]),
+    "vkb_context_selftest_stalled_kernel": (C.c_int, [P, U32]),
     "vkb_kv_release_seq": (C.c_int, [P, I32]),
     "vkb_kv_release_layer": (C.c_int, [P, I32]),
     "vkb_kv_reset": (C.c_int, [P]),

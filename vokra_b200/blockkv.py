@@ -19,6 +19,7 @@ The context's stream is the one that was torch's current stream when the context
 was made (Context.set_stream changes it). Tensors that were written, or are read
 or freed, on another stream are ordered by the caller, with an event, as for any
 other kernel; a tensor that a call allocates belongs to torch's current stream.
+Waits inside the kernels are bounded: ctx.synchronize() raises where one gave up and a result is not complete.
 A whole decode loop is in examples/beam_decode.py.
 """
 from __future__ import annotations

@@ -1,5 +1,6 @@
 // context.cu — library-level entry points: last error, ABI version, context.
 #include "common.cuh"
+#include "linear.cuh"
 #include <cstdlib>
 #include <cstdio>
 
@@ -73,6 +74,8 @@ vkb_status vkb_context_synchronize(vkb_context* ctx) {
         if (!ctx) fail(VKB_ERROR_INVALID_ARGUMENT, "synchronize: null context");
         VKB_CUDA(cudaStreamSynchronize(ctx->stream));
         VKB_CUDA(cudaGetLastError());
+        if (read_and_clear_err_flag(ctx))
+            fail(VKB_ERROR_OTHER, "synchronize: a wait in a kernel gave up; a result since the last synchronize is not complete");
     });
 }
 

@@ -1464,7 +1464,7 @@ vkb_status vkb_gemm_q_f32(vkb_context* ctx, int64_t m, int64_t n, int64_t k, con
                    VKB_EPI_NONE, nullptr, 1.0f, nullptr, nullptr);
         VKB_CUDA(cudaMemcpyAsync(out_host, o.p, o.n, cudaMemcpyDeviceToHost, ctx->stream));
         VKB_CUDA(cudaStreamSynchronize(ctx->stream));
-        if (read_and_clear_err_flag(ctx)) fail(VKB_ERROR_OTHER, "gemm_q_f32: a pipeline wait timed out on the device");
+        if (read_and_clear_err_flag(ctx)) fail(VKB_ERROR_OTHER, "gemm_q_f32: a pipeline wait timed out on the device, in this call or in one since the last synchronize");
     });
 }
 
@@ -1479,6 +1479,16 @@ vkb_status vkb_context_selftest_bounded_wait(vkb_context* ctx, uint32_t polls) {
         ctx->count();
         if (read_and_clear_err_flag(ctx)) fail(VKB_ERROR_OTHER, "selftest_bounded_wait: the wait gave up after " +
                                                                     std::to_string(polls) + " polls");
+    });
+}
+
+vkb_status vkb_context_selftest_stalled_kernel(vkb_context* ctx, uint32_t polls) {
+    return guard([&] {
+        if (!ctx) fail(VKB_ERROR_INVALID_ARGUMENT, "selftest_stalled_kernel: null context");
+        if (polls == 0 || polls > (1u << 20)) fail(VKB_ERROR_INVALID_ARGUMENT, "selftest_stalled_kernel: polls in 1..2^20");
+        bounded_wait_selftest_kernel<<<1, 32, 0, ctx->stream>>>(device_err_flag(ctx), polls);
+        VKB_CUDA(cudaGetLastError());
+        ctx->count();
     });
 }
 

@@ -50,6 +50,7 @@ class Context:
         check(_L.vkb_context_set_stream(self.h, C.c_void_p(stream_handle) if stream_handle else None))
 
     def synchronize(self):
+        """Waits for the stream; raises where a wait inside a kernel since the last call gave up."""
         check(_L.vkb_context_synchronize(self.h))
 
     @property
