@@ -133,9 +133,11 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (M::BARS + 7) / 8 * 8);
     uint64_t *q_full = bars, *k_full = bars + 1, *v_full = bars + 3, *k_empty = bars + 5, *v_empty = bars + 7;
     uint64_t *s_full = bars + 9, *p_full = bars + 13, *pv_done = bars + 17;  // [tile * 2 + half]
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+    uint64_t* ended = bars + 21;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
     if (threadIdx.x == 0) {
         ptx::mbar_init(q_full, 256);
+        ptx::mbar_init(ended, 1);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&k_full[i], 128);
             ptx::mbar_init(&v_full[i], 96);
@@ -382,6 +384,9 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             }
             ids_next = ids_of(j + 2);
         }
+        // The last steps' buffers are given back too: the block does not end before those arrivals.
+        for (int j = max(0, n_steps - 2); j < n_steps && ok; ++j)
+            if (2 * j + 1 < n_half && !ptx::mbar_wait(&empty[j & 1], (j >> 1) & 1)) ok = false;
     } else if (n_steps > 0) {
         // ---- the products, by the whole warp in step. Half i of a tile's keys has its scores in half i % 2 of the tile's
         // columns, so S of the next half is made while this one's softmax runs. Tile t is at S of half s_at[t] and P.V of
@@ -437,7 +442,14 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             }
         }
     }
-    if (!ok) atomicExch(err, 1);
+    if (!ok) {
+        atomicExch(err, 1);
+        // products under way end before the block does
+        if (warp == 15) {
+            ptx::mma_commit_warp(ended);
+            ptx::mbar_wait(ended, 0);
+        }
+    }
     __syncwarp();
     ptx::tc_fence_before();
     __syncthreads();
