@@ -110,7 +110,7 @@ def beam_search(model, prompts, beams, steps, eot, repetition=1.2, no_repeat_ngr
     n_new = torch.tensor(lens, dtype=torch.int32, device=dev)
     history_len.copy_(n_new)
     pages.advance(a, b, None, n_new)
-    batch = Batch(start, b.len, b.table, sum(lens), max(lens), status)
+    batch = Batch(start, b.len, b.table, sum(lens), max(lens), status, max_kv=max(lens))
     tokens = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=dev)
     last = (start[1:] - 1).clamp(min=0).long()
     x = model.step(cache, batch, tokens, last)

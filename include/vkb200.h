@@ -547,6 +547,8 @@ typedef struct vkb_bkv_batch {
     const int32_t* table_dev;      /* [n_seq][table_ld] */
     int64_t table_ld;
     const int32_t* status_dev;     /* NULL, or vkb_pages_advance's status: where it is not 0, nothing is appended */
+    int32_t max_kv;                /* tokens of the longest stream, 0 = unknown (a hint like max_q; without it the width
+                                    * of the table stands for it) */
 } vkb_bkv_batch;
 
 /* Stores the batch's rows of K and V ([n_tok] rows of n_kv_head*d_head values,

@@ -207,3 +207,39 @@ def test_rows_of_tiny_values(ctx, size, d):
     got = run(ctx, plain, table, [0, 5], lens, q, scale=0.125 / (size * up)).astype(np.float64)
     want, size_of, _ = exact(plain, table, [0, 5], lens, q, np.float64(np.float32(0.125 / (size * up))))
     assert (np.abs(got - want).max(2) <= REL["float32"] * size_of).all()
+
+
+def test_a_wider_table_takes_the_same_kernel(ctx):
+    """A table with room for more tokens than the streams have: same pages, same bits."""
+    rng = np.random.default_rng(14)
+    heads, group, d = 8, 4, 128
+    lens, new = [2000, 700], [2000, 500]
+    start = np.concatenate([[0], np.cumsum(new)])
+    table, n_pages = tables(rng, lens)
+    cache = cache_of(ctx, filled(rng, n_pages, heads, d))
+    q = dev(rng.standard_normal((start[-1], heads * group, d)).astype(np.float16))
+    first = cache.attention(0, batch_of(table, start, lens), q, d**-0.5).cpu().numpy()
+    for times in (2, 8, 64):
+        wide = np.full((2, times * table.shape[1]), -1, np.int32)
+        wide[:, :table.shape[1]] = table
+        assert np.array_equal(cache.attention(0, batch_of(wide, start, lens), q, d**-0.5).cpu().numpy(), first)
+
+
+def test_a_wider_table_of_few_rows_with_a_hint(ctx):
+    """Few enough rows that the number of keys decides: max_kv says it where the table does not."""
+    from vokra_b200 import blockkv
+    rng = np.random.default_rng(15)
+    heads, group, d, n, new = 8, 4, 128, 1000, 100
+    table, n_pages = tables(rng, [n])
+    cache = cache_of(ctx, filled(rng, n_pages, heads, d))
+    q = dev(rng.standard_normal((new, heads * group, d)).astype(np.float16))
+    wide = np.full((1, 4096), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    i32 = lambda *x: dev(np.array(x, np.int32))  # noqa: E731
+    got = [cache.attention(0, blockkv.Batch(i32(0, new), i32(n), dev(t), new, new, max_kv=kv), q, d**-0.5).cpu().numpy()
+           for t, kv in ((table, 0), (wide, n), (wide, 0), (table, n))]
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[3])
+    # without the hint it is another kernel, and the same values to its rounding (2 * 2^-11 of values up to 4.5)
+    assert np.abs(got[0].astype(np.float64) - got[2]).max() <= 2 * 4.5e-3
+    with pytest.raises(blockkv.VkbError):
+        cache.attention(0, blockkv.Batch(i32(0, new), i32(n), dev(table), new, new, max_kv=-1), q)

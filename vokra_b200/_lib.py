@@ -99,7 +99,8 @@ class BkvCache(C.Structure):
 
 class BkvBatch(C.Structure):
     _fields_ = [("n_seq", C.c_int32), ("n_tok", C.c_int32), ("max_q", C.c_int32), ("tok_start", C.c_void_p),
-                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int64), ("status", C.c_void_p)]
+                ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_ld", C.c_int64), ("status", C.c_void_p),
+                ("max_kv", C.c_int32)]
 
 
 class PagePlane(C.Structure):

@@ -46,9 +46,10 @@ class Batch:
     """The streams of a step: stream s owns rows tok_start[s] .. tok_start[s + 1] - 1 of the step's row
     tensors, which are its last rows; kv_len[s] counts its tokens, the step's included; table[s] lists its
     pages. n_tok = tok_start[-1], max_q the largest number of rows of a stream; status (optional): the
-    status of PagePool, append stores nothing where it is not 0."""
+    status of PagePool, append stores nothing where it is not 0; max_kv (optional): tokens of the longest
+    stream, for the choice of the attention's kernel (0: as many as the table holds)."""
 
-    def __init__(self, tok_start, kv_len, table, n_tok: int, max_q: int, status=None):
+    def __init__(self, tok_start, kv_len, table, n_tok: int, max_q: int, status=None, max_kv: int = 0):
         s = _lib.BkvBatch()
         s.tok_start, s.kv_len, s.table = _i32(tok_start, "tok_start", 1), _i32(kv_len, "kv_len", 1), _i32(table, "table", 2)
         if not tok_start.is_contiguous() or not kv_len.is_contiguous():
@@ -56,7 +57,7 @@ class Batch:
         n_seq = kv_len.shape[0]
         if tok_start.shape[0] != n_seq + 1 or table.shape[0] != n_seq:
             _bad(f"{n_seq} lengths want {n_seq + 1} starts and {n_seq} rows of the table")
-        s.n_seq, s.n_tok, s.max_q = n_seq, n_tok, max_q
+        s.n_seq, s.n_tok, s.max_q, s.max_kv = n_seq, n_tok, max_q, max_kv
         s.table_ld = table.stride(0) if n_seq > 1 else table.shape[1]
         if s.table_ld != table.shape[1]:
             _bad("table: its rows must follow one another")

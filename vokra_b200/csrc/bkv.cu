@@ -45,7 +45,7 @@ BkvLayer bkv_layer(const vkb_context* ctx, const vkb_bkv_cache* c, int layer) {
 
 BkvStreams bkv_streams(const vkb_bkv_batch* b) {
     if (!b) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv: null batch");
-    if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv: negative count in the batch");
+    if (b->n_seq < 0 || b->n_tok < 0 || b->max_q < 0 || b->max_kv < 0) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv: negative count in the batch");
     if (b->n_seq > VKB_BKV_MAX_SEQ)
         fail(VKB_ERROR_UNSUPPORTED_OP, "bkv: more than " + std::to_string(VKB_BKV_MAX_SEQ) + " streams in one call");
     if (b->n_seq && (!b->tok_start_dev || !b->kv_len_dev || !b->table_dev))

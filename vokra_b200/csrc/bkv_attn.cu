@@ -907,6 +907,7 @@ extern "C" vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* c
         a.group = n_head / cache->n_kv_head;
         a.n_head = n_head;
         a.max_q = std::max(1, std::min(batch->max_q, batch->n_tok));
+        a.max_kv = batch->max_kv;
         if ((int64_t)batch->n_tok * a.group > INT32_MAX / 2) fail(VKB_ERROR_UNSUPPORTED_OP, "bkv_attention: too many rows");
         a.q_f16 = q_dtype == VKB_DT_F16;
         a.out_f16 = out_dtype == VKB_DT_F16;

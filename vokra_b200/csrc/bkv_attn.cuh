@@ -9,6 +9,7 @@ struct BkvAttn {
     BkvLayer L;
     BkvStreams S;
     int d_head, group, n_head, max_q;
+    int max_kv;  // tokens of the longest stream; 0: not known
     const void* q;
     int64_t q_ld;
     float scale;

@@ -29,6 +29,7 @@
 // above fp32's smallest number in the sum.
 #include "bkv_attn.cuh"
 #include "tc_ptx.cuh"
+#include <algorithm>
 
 namespace vkb {
 namespace {
@@ -479,18 +480,25 @@ void launch(vkb_context* ctx, const BkvAttn& a) {
 bool bkv_prompt_takes(const vkb_context* ctx, const BkvAttn& a) {
     if (!a.q_f16 || !a.out_f16 || (a.d_head != 64 && a.d_head != 128)) return false;
     if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_ld % 8 || a.out_ld % 8) return false;
-    // A wave of these blocks takes the time of its longest stream whatever the rows; the other kernel's grows with the
-    // rows and less with the keys. Microseconds here and there, 8 KV heads of 128, group 4, one stream:
-    //   500 keys, 16 rows 16 and 20; 64 rows 20 and 20          (tables of up to 32 pages: here)
-    //   1000 keys, 64 rows 29 and 28; 128 rows 30 and 36        (128 and 256 tiles of 16 rows, all heads)
-    //   2000 keys, 64 rows 49 and 31; 128 rows 50 and 45        (128 and 256 tiles)
-    //   4000 keys, 128 rows 87 and 67; 256 rows 87 and 111      (256 and 512 tiles)
-    // 8 heads of 64, 1000 keys: 128 tiles 26 and 23, 256 tiles 26 and 27; 20 heads, 2000 keys: 320 tiles 45 and 39.
+    // A wave of these blocks takes the time of its longest stream whatever the rows. The other kernel's time grows with the
+    // rows, by tiles of 16 (all heads), and has a fixed part that counts with few keys: what this one needs to be the faster
+    // is tiles for each of its waves, more of them the more keys there are, up to as many as make the two grow alike.
+    // Microseconds here and there, one stream, group 4, 8 KV heads:
+    //   d_head 128, 1000 keys:  128 tiles 35 and 33, 256 tiles 35 and 41
+    //               2000        256 tiles 55 and 51, 512 tiles 55 and 76
+    //               4000        256 tiles 96 and 74, 512 tiles 95 and 117
+    //               64000       256 tiles 1294 and 659, 512 tiles 1292 and 1295, 1024 tiles 1294 and 2534
+    //   d_head 64,  1000        128 tiles 29 and 28, 256 tiles 30 and 33
+    //               4000        512 tiles 82 and 80, 1024 tiles 84 and 131
+    //               64000       512 tiles 1146 and 780, 1024 tiles 1147 and 1518
+    // Up to 512 keys: 500 keys, 16 rows 16 and 20; 64 rows 20 and 20. Where the longest stream is not known the table's
+    // width stands for it, which matters below the upper limit only (1.7 times the time at worst: 1000 keys).
     if ((int64_t)a.max_q * a.group < 64) return false;
-    if (a.S.ld <= 32) return true;
+    const int64_t pages = a.max_kv > 0 ? std::min<int64_t>(a.S.ld, ((int64_t)a.max_kv + BKV_BLOCK - 1) / BKV_BLOCK) : a.S.ld;
+    if (pages <= 32) return true;
     const int64_t blocks = most_tiles(a) * a.L.n_kv_head, waves = (blocks + ctx->sm_count - 1) / ctx->sm_count;
     const int64_t tiles = ((int64_t)a.S.n_tok * a.group + 15) / 16 * a.L.n_kv_head;
-    return tiles >= waves * a.S.ld * (a.d_head == 64 ? 4 : 2);
+    return tiles >= waves * (a.d_head == 64 ? std::min<int64_t>(4 * pages, 768) : std::min<int64_t>(2 * pages, 512));
 }
 
 void run_bkv_prompt(vkb_context* ctx, const BkvAttn& a) {
