@@ -476,7 +476,7 @@ VKB_API vkb_status vkb_log_mel(vkb_context* ctx, const float* pcm_dev, int64_t n
 typedef struct vkb_logits_rules {
     const int32_t* hist_dev;       /* [rows][hist_ld] token ids; ids outside the vocabulary count for nothing */
     int64_t hist_ld;
-    const int32_t* hist_len_dev;   /* [rows] valid ids of each row (clipped to hist_ld); NULL = hist_ld */
+    const int32_t* hist_len_dev;   /* [rows] valid ids of each row (clipped to hist_cols); NULL = hist_cols */
     const float* repetition_dev;   /* [rows] */
     const float* frequency_dev;    /* [rows] */
     const float* presence_dev;     /* [rows] */
@@ -489,6 +489,7 @@ typedef struct vkb_logits_rules {
     int64_t mask_ld;
     const int32_t* mask_row_dev;   /* [rows]; outside 0..n_mask-1 = no mask; NULL = row 0 for every row */
     int32_t n_mask;
+    int64_t hist_cols;             /* ids of a row of hist_dev, where rows are parts of longer ones; 0 = hist_ld */
 } vkb_logits_rules;
 
 /* out[r][j] = the logits after the rules (NULL rules: a copy), rounded once to

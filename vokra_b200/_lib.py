@@ -83,7 +83,7 @@ class LogitsRules(C.Structure):
         ("hist", C.c_void_p), ("hist_ld", C.c_int64), ("hist_len", C.c_void_p), ("repetition", C.c_void_p),
         ("frequency", C.c_void_p), ("presence", C.c_void_p), ("no_repeat_ngram", C.c_int32), ("n_bias", C.c_int32),
         ("bias", C.c_void_p), ("bias_ld", C.c_int64), ("bias_row", C.c_void_p), ("mask", C.c_void_p),
-        ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("n_mask", C.c_int32),
+        ("mask_ld", C.c_int64), ("mask_row", C.c_void_p), ("n_mask", C.c_int32), ("hist_cols", C.c_int64),
     ]
 
 

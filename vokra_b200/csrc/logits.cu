@@ -42,7 +42,7 @@ __device__ __forceinline__ float ex2(float x) {
 
 struct Rules {
     const int32_t* hist;
-    int64_t hist_ld;
+    int64_t hist_ld, hist_cols;
     const int32_t* hist_len;
     const float *rep, *freq, *pres;
     int ngram;
@@ -68,8 +68,8 @@ struct RowRules {
         n_hist = 0;
         if (R.hist) {
             hist = R.hist + (int64_t)row * R.hist_ld;
-            const int64_t n = R.hist_len ? (int64_t)R.hist_len[row] : R.hist_ld;
-            n_hist = (int)(n < 0 ? 0 : n > R.hist_ld ? R.hist_ld : n);
+            const int64_t n = R.hist_len ? (int64_t)R.hist_len[row] : R.hist_cols;
+            n_hist = (int)(n < 0 ? 0 : n > R.hist_cols ? R.hist_cols : n);
         }
         rep = R.rep ? R.rep[row] : 1.0f;
         freq = R.freq ? R.freq[row] : 0.0f;
@@ -708,6 +708,7 @@ Rules check_rules(const vkb_logits_rules* r, int64_t vocab) {
     Rules R{};
     if (!r) return R;
     if (r->hist_ld < 0) fail(VKB_ERROR_INVALID_ARGUMENT, "logits: negative hist_ld");
+    if (r->hist_cols < 0 || r->hist_cols > r->hist_ld) fail(VKB_ERROR_INVALID_ARGUMENT, "logits: hist_cols must be in 0..hist_ld");
     if (r->hist_len_dev && !r->hist_dev) fail(VKB_ERROR_INVALID_ARGUMENT, "logits: history lengths without a history");
     if (r->hist_ld > INT32_MAX) fail(VKB_ERROR_UNSUPPORTED_OP, "logits: history longer than 2^31 - 1");
     if (r->no_repeat_ngram < 0) fail(VKB_ERROR_INVALID_ARGUMENT, "logits: negative no_repeat_ngram");
@@ -717,6 +718,7 @@ Rules check_rules(const vkb_logits_rules* r, int64_t vocab) {
         fail(VKB_ERROR_INVALID_ARGUMENT, "logits: the mask table needs n_mask >= 1 rows of at least ceil(n_vocab / 32) words");
     R.hist = r->hist_ld > 0 ? r->hist_dev : nullptr;
     R.hist_ld = r->hist_ld;
+    R.hist_cols = r->hist_cols ? r->hist_cols : r->hist_ld;
     R.hist_len = r->hist_len_dev;
     R.rep = r->repetition_dev;
     R.freq = r->frequency_dev;

@@ -64,8 +64,9 @@ class LogitsRules:
         s = _lib.LogitsRules()
         s.hist = _tensor(history, "history", i32, 2)
         s.hist_ld = 0 if history is None else _ld(history) if history.shape[1] else 0
-        if history is not None and (s.hist_ld < history.shape[1] or s.hist_ld > history.shape[1] and history_len is None):
-            _bad("history: its rows overlap, or are part of longer ones and have no history_len")
+        if history is not None and s.hist_ld < history.shape[1]:
+            _bad("history: its rows overlap")
+        s.hist_cols = 0 if history is None else history.shape[1]
         s.hist_len = _tensor(history_len, "history_len", i32, 1)
         s.repetition = _tensor(repetition, "repetition", f32, 1)
         s.frequency = _tensor(frequency, "frequency", f32, 1)
