@@ -30,7 +30,7 @@ import torch
 
 from . import _lib
 from ._lib import check, VkbError  # noqa: F401
-from .logits import _DTYPES, _bad, _tensor
+from .logits import _DTYPES, _at_home, _bad, _device, _tensor
 
 _L = _lib.load()
 BLOCK = _lib.BKV_BLOCK
@@ -64,6 +64,7 @@ class Batch:
         s.status = None if status is None else _i32(status, "status", 1)
         self.n_tok = n_tok
         self.tensors = (tok_start, kv_len, table, status)
+        self.device = _device(self.tensors)
         self.struct, self.ref = s, C.byref(s)
 
 
@@ -78,6 +79,7 @@ class PageState:
             _bad("a page state's tensors must be contiguous")
         if len.shape[0] != table.shape[0]:
             _bad("as many lengths as rows of the table are wanted")
+        self.device = _device((table, len, refs))
         self.struct, self.ref = s, C.byref(s)
 
     @staticmethod
@@ -99,6 +101,7 @@ class PagePool:
                 _bad(f"arenas: contiguous CUDA tensors of shape [{n_layer}, {n_pages}, ...] are wanted")
             page = t.element_size() * (t.numel() // (n_layer * n_pages))
             p.base, p.page_bytes, p.layer_bytes = t.data_ptr(), page, page * n_pages
+        _at_home(ctx, _device((*arenas, status)), "arenas and status")
         self.ctx, self.status, self.n_pages = ctx, status, n_pages
         self._keep = (arenas, planes)
         self.struct = _lib.PagePool(n_layer, len(arenas), planes, n_pages, 0, page_tokens, 0, _i32(status, "status", 1))
@@ -107,6 +110,8 @@ class PagePool:
     def _states(self, a: PageState, b: PageState):
         if a.table.shape != b.table.shape or a.refs.shape != b.refs.shape or a.refs.shape[0] != self.n_pages:
             _bad("pages: the two states have other shapes than each other or than the arenas")
+        _at_home(self.ctx, a.device, "state")
+        _at_home(self.ctx, b.device, "state")
         self.struct.n_seq, self.struct.table_ld = a.table.shape
 
     def advance(self, a: PageState, b: PageState, parent=None, n_new=None):
@@ -117,12 +122,16 @@ class PagePool:
         for t, name in ((parent, "parent"), (n_new, "n_new")):
             if t is not None and (_i32(t, name, 1) is None or t.shape[0] != a.len.shape[0] or not t.is_contiguous()):
                 _bad(f"{name}: a contiguous int32 tensor with one entry a stream is wanted")
+            if t is not None:
+                _at_home(self.ctx, t.get_device(), name)
         check(_L.vkb_pages_advance(self.ctx.h, self.ref, None if parent is None else parent.data_ptr(),
                                    None if n_new is None else n_new.data_ptr(), a.ref, b.ref))
 
     def compact(self, a: PageState, b: PageState, n_used=None):
         """b = a with the pages in use moved to the front of the arenas; n_used (int32 [1]): how many there are."""
         self._states(a, b)
+        if n_used is not None:
+            _at_home(self.ctx, n_used.get_device(), "n_used")
         check(_L.vkb_pages_compact(self.ctx.h, self.ref, a.ref, b.ref, None if n_used is None else _i32(n_used, "n_used", 1)))
 
     def check(self):
@@ -150,6 +159,7 @@ class BlockKvCache:
                 _bad(f"{name} must be [n_layer, n_pages, n_kv_head]")
         if not all(t.is_contiguous() for t in (k, v, k_scale, v_scale)):
             _bad("the arenas must be contiguous")
+        _at_home(ctx, _device((k, v, k_scale, v_scale)), "arenas")
         self.ctx, self.k, self.v, self.k_scale, self.v_scale = ctx, k, v, k_scale, v_scale
         self.n_layer, self.n_pages, self.n_kv_head, self.d_head = n_layer, n_pages, n_kv_head, d_head
         self.struct = _lib.BkvCache(n_layer, n_kv_head, d_head, n_pages, k.data_ptr(), v.data_ptr(), k_scale.data_ptr(),
@@ -180,6 +190,10 @@ class BlockKvCache:
             ok = len(shape) == 2 and shape[1] == heads * d and stride[1] == 1
         if not ok or shape[0] < batch.n_tok or not t.is_cuda:
             _bad(f"{name}: CUDA rows [{batch.n_tok}, {heads}, {d}] with contiguous rows are wanted, got {tuple(shape)}")
+        on = t.get_device()
+        if on != self.ctx.device or batch.device != on:
+            _at_home(self.ctx, on, name)
+            _at_home(self.ctx, batch.device, "batch")
         return t.data_ptr(), stride[0] if shape[0] > 1 else heads * d, dt
 
     def append(self, layer: int, batch: Batch, k, v):
@@ -212,6 +226,7 @@ class BlockKvCache:
         dt = _DTYPES.get(dtype)
         if dt is None:
             _bad(f"read: dtype must be f32 or f16, got {dtype}")
+        _at_home(self.ctx, batch.device, "batch")
         k = torch.empty((batch.n_tok, self.n_kv_head, self.d_head), dtype=dtype, device=self.k.device)
         v = torch.empty_like(k)
         status = _L.vkb_bkv_read(self.ctx.h, self.ref, layer, batch.ref, k.data_ptr(), v.data_ptr(), dt)

@@ -44,6 +44,20 @@ def _tensor(t, name: str, dtypes, ndim: int):
     return t.data_ptr()
 
 
+def _device(tensors) -> int | None:
+    """The GPU that all of these (None among them) are on; None where there is no tensor."""
+    on = {t.get_device() for t in tensors if t is not None}
+    if len(on) > 1:
+        _bad(f"tensors of one call on different GPUs: {sorted(on)}")
+    return on.pop() if on else None
+
+
+def _at_home(ctx, device, name: str):
+    """Refuses tensors of another GPU than the context's."""
+    if device is not None and device != ctx.device:
+        _bad(f"{name}: on GPU {device}, the context is on GPU {ctx.device}")
+
+
 def _ld(t) -> int:
     """The stride between rows, in elements; at least a row where there is one row only (its stride says nothing)."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -86,13 +100,16 @@ class LogitsRules:
         self._bias_width = None if bias is None else bias.shape[1]
         self._mask_words = None if mask is None else mask.shape[1]
         self._checked = None
+        self.device = _device(self.tensors)
         self.struct = s
         self.ref = C.byref(s)
 
-    def check(self, rows: int, vocab: int):
-        """Whether the rules fit a batch of this shape."""
-        if self._checked == (rows, vocab):
+    def check(self, rows: int, vocab: int, device: int | None = None):
+        """Whether the rules fit a batch of this shape, on this GPU (None: whichever they are on)."""
+        if self._checked == (rows, vocab, device):
             return
+        if device is not None and self.device is not None and self.device != device:
+            _bad(f"rules: on GPU {self.device}, the context is on GPU {device}")
         for name, t in self._per_row:
             if t.shape[0] < rows:
                 _bad(f"{name}: {t.shape[0]} rows for {rows} rows of logits")
@@ -100,7 +117,7 @@ class LogitsRules:
             _bad(f"bias: rows of {self._bias_width} values for a vocabulary of {vocab}")
         if self._mask_words is not None and self._mask_words < (vocab + 31) // 32:
             _bad(f"mask: rows of {self._mask_words} words for a vocabulary of {vocab}")
-        self._checked = (rows, vocab)
+        self._checked = (rows, vocab, device)
 
 
 _DTYPES = {torch.float32: _lib.DT_F32, torch.float16: _lib.DT_F16}
@@ -121,6 +138,8 @@ def _matrix(t, name: str):
 def process(ctx, logits, rules: LogitsRules | None = None, out=None):
     """The logits ([rows, vocab], f32 or f16) after the rules, in their own type; out may be logits."""
     p, dt, rows, vocab, ld = _matrix(logits, "logits")
+    if logits.get_device() != ctx.device:
+        _at_home(ctx, logits.get_device(), "logits")
     if out is None:
         out = torch.empty((rows, vocab), dtype=logits.dtype, device=logits.device)
         to, out_ld = out.data_ptr(), vocab
@@ -128,10 +147,11 @@ def process(ctx, logits, rules: LogitsRules | None = None, out=None):
         to, out_dt, out_rows, out_vocab, out_ld = _matrix(out, "out")
         if (out_rows, out_vocab, out_dt) != (rows, vocab, dt):
             _bad("out: another shape or dtype than logits")
+        _at_home(ctx, out.get_device(), "out")
     ref = None
     if rules is not None:
-        if rules._checked != (rows, vocab):
-            rules.check(rows, vocab)
+        if rules._checked != (rows, vocab, ctx.device):
+            rules.check(rows, vocab, ctx.device)
         ref = rules.ref
     status = _L.vkb_logits_process(ctx.h, p, dt, rows, vocab, ld, ref, to, out_ld)
     if status:
@@ -143,19 +163,23 @@ def topk(ctx, logits, k: int, rules: LogitsRules | None = None, ids=None, logpro
     """(ids int32 [rows, k], log-probabilities f32 [rows, k]) of the k best tokens after the rules, the
     best first, ties by the lower id; id -1 at -inf where fewer than k tokens are left."""
     p, dt, rows, vocab, ld = _matrix(logits, "logits")
+    if logits.get_device() != ctx.device:
+        _at_home(ctx, logits.get_device(), "logits")
     if not 1 <= k <= TOPK_MAX:
         _bad(f"k must be in 1..{TOPK_MAX}, got {k}")
     for t, name, dtype in ((ids, "ids", torch.int32), (logprobs, "logprobs", torch.float32)):
         if t is not None and (t.dtype != dtype or tuple(t.shape) != (rows, k) or not t.is_contiguous() or not t.is_cuda):
             _bad(f"{name}: a contiguous {dtype} CUDA tensor of shape [{rows}, {k}] is wanted")
+        if t is not None:
+            _at_home(ctx, t.get_device(), name)
     if ids is None:
         ids = torch.empty((rows, k), dtype=torch.int32, device=logits.device)
     if logprobs is None:
         logprobs = torch.empty((rows, k), dtype=torch.float32, device=logits.device)
     ref = None
     if rules is not None:
-        if rules._checked != (rows, vocab):
-            rules.check(rows, vocab)
+        if rules._checked != (rows, vocab, ctx.device):
+            rules.check(rows, vocab, ctx.device)
         ref = rules.ref
     status = _L.vkb_logits_topk(ctx.h, p, dt, rows, vocab, ld, ref, k, ids.data_ptr(), logprobs.data_ptr())
     if status:
