@@ -52,3 +52,23 @@ def test_tensors_of_another_gpu(ctx):
             call()
         assert e.value.code == _lib.ERROR_INVALID_ARGUMENT, n
     assert ctx.launch_count == launches
+
+
+def test_more_refusals(ctx):
+    """Shapes that ended in errors of another kind, and a scale whose products leave fp32."""
+    import torch
+    from vokra_b200 import _lib, blockkv
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    cache = blockkv.BlockKvCache.empty(ctx, 1, 2, 64, 4)
+    batch = blockkv.Batch(i(2), i(1), i(1, 4), 1, 1)
+    q = torch.zeros(1, 4, 64, device="cuda")
+    for n, call in enumerate([
+        lambda: cache.attention(0, batch, q[0, 0]), lambda: cache.attention(0, batch, q[0, 0, 0]), lambda: cache.attention(0, batch, q[None]),
+        lambda: cache.append(0, batch, q[0, 0], q[0, 0]), lambda: cache.attention(0, batch, q, scale=2.5e38),
+        lambda: blockkv.PagePool(ctx, [], i(1)), lambda: blockkv.PagePool(ctx, [torch.zeros(2, 0, 4, device="cuda")], i(1)),
+        lambda: blockkv.PagePool(ctx, [torch.zeros(8, device="cuda")], i(1)),
+    ]):
+        with pytest.raises(blockkv.VkbError) as e:
+            call()
+        assert e.value.code == _lib.ERROR_INVALID_ARGUMENT, n
+    cache.attention(0, batch, q, scale=1.9e38)

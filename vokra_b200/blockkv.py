@@ -94,6 +94,8 @@ class PagePool:
     """The pages of one or more arenas [n_layer, n_pages, ...], contiguous tensors of any type."""
 
     def __init__(self, ctx, arenas, status, page_tokens: int = BLOCK):
+        if not arenas or any(t.dim() < 2 or not t.numel() for t in arenas):
+            _bad("arenas: one tensor of pages at least, none of them empty, is wanted")
         n_layer, n_pages = arenas[0].shape[:2]
         planes = (_lib.PagePlane * len(arenas))()
         for p, t in zip(planes, arenas):
@@ -208,7 +210,7 @@ class BlockKvCache:
 
     def attention(self, layer: int, batch: Batch, q, scale: float = 1.0, out=None):
         """Causal attention of the rows q [n_tok, n_head, d_head] over their streams' caches; out like q unless given."""
-        heads = q.shape[1] if q.dim() == 3 else q.shape[1] // self.d_head
+        heads = q.shape[1] if q.dim() == 3 else q.shape[-1] // self.d_head if q.dim() else 0
         qp, q_ld, q_dt = self._rows(q, "q", heads, batch)
         if out is None:
             out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

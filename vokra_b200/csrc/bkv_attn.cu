@@ -901,7 +901,8 @@ extern "C" vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* c
         a.d_head = cache->d_head;
         const int64_t width = (int64_t)n_head * a.d_head;
         if (q_ld < width || out_ld < width) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: row stride below n_head*d_head");
-        if (!(scale > 0.0f) || scale > 3.0e38f) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: scale must be positive and finite");
+        if (!(scale > 0.0f) || scale > 2.0e38f)  // (times log2(e) it is finite)
+            fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: scale must be positive and at most 2e38");
         if (batch->n_seq == 0 || batch->n_tok == 0) return;
         if (!q_dev || !out_dev) fail(VKB_ERROR_INVALID_ARGUMENT, "bkv_attention: null q/out");
         a.group = n_head / cache->n_kv_head;
