@@ -539,8 +539,8 @@ typedef struct vkb_bkv_cache {
  * position kv_len[s] - 1. Page p of the stream is table[s * table_ld + p]; an id
  * outside 0..n_pages-1 is a page that is not there: it is never written, and
  * its tokens are not seen. n_tok = tok_start[n_seq]; max_q is the largest
- * number of rows of one stream (a hint for the choice of kernels: a wrong one
- * costs time). */
+ * number of rows of one stream (for the choice of kernels: a wrong one costs
+ * time, and with F16 rows the last bits, see vkb_bkv_attention). */
 typedef struct vkb_bkv_batch {
     int32_t n_seq, n_tok, max_q;
     const int32_t* tok_start_dev;  /* [n_seq + 1] */
@@ -567,10 +567,22 @@ VKB_API vkb_status vkb_bkv_append(vkb_context* ctx, const vkb_bkv_cache* cache, 
  * out = softmax(scale * q . K) V per head, over the keys at positions up to the
  * row's own. Query head j reads KV head j / (n_head / n_kv_head). q and out:
  * [n_tok] rows of n_head*d_head values, row strides in elements, F32 or F16
- * each. With an F32 q or out the products are accurate to about 2^-21, else
- * q and the weights enter them as f16; sums and statistics are fp32 either
- * way. A row without keys (a stream of length 0) is zero; a row of q with an
- * infinity or NaN is NaN. */
+ * each. `scale` is above 0 and at most 2e38. A row that sees no key is zero,
+ * whatever it holds; one with an infinity or NaN that sees a key is NaN.
+ *
+ * Bits. Sums and softmax statistics are fp32. q is known to a part of its row's
+ * largest value, weights to a part of themselves:
+ *   an F32 q or out             q 2^-24, weights 2^-21
+ *   F16, max_q * group <= 8     q 2^-16, weights 2^-21
+ *   F16, more rows              q 2^-16, weights 2^-11
+ *   F16, prompts (d_head 64 or 128, 64 rows or more, chosen by sizes)
+ *                               q as it is, weights 2^-11
+ * so with F16 q and out max_q and max_kv, which choose among these, decide the
+ * last bits too. Weights below 2^-28 (prompts: 2^-21) of the row's largest
+ * product of weight and V scale lose bits to a fixed step. Blocks that a row does
+ * not see do not matter to it, whatever they hold; among those that it sees V
+ * scales up to 2^100 apart leave the weights' sum right (prompts: scales below
+ * 2^-60, whose values are 0 in f16, count as 2^-60 in the products). */
 VKB_API vkb_status vkb_bkv_attention(vkb_context* ctx, const vkb_bkv_cache* cache, int32_t layer,
                                      const vkb_bkv_batch* batch, int32_t n_head, const void* q_dev, int64_t q_ld,
                                      int32_t q_dtype, float scale, void* out_dev, int64_t out_ld, int32_t out_dtype);

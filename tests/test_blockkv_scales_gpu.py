@@ -209,6 +209,26 @@ def test_rows_of_tiny_values(ctx, size, d):
     assert (np.abs(got - want).max(2) <= REL["float32"] * size_of).all()
 
 
+@pytest.mark.parametrize("dtype,new,group", FORMS)
+def test_rows_with_an_outlying_channel(ctx, dtype, new, group):
+    """One channel of q is 200 and the others about 1. The kernel for few rows takes 16-bit rows of q to 2^-15.98 of the
+    row's largest value and 32-bit rows to 2^-23.97, the tensor-core tiles take them as they are. Errors of a uniform
+    distribution over 64 channels and |k| of 1.75 (root of the mean square), six times over, move a score by at most
+    `off`, its weight by that part, and the sum of the weights too."""
+    rng = np.random.default_rng(13)
+    heads, d, lens = 2, 64, [300]
+    table, n_pages = tables(rng, lens)
+    plain = filled(rng, n_pages, heads, d)
+    plain.k[:, :, :, 9] = 1
+    q = rng.standard_normal((new, heads * group, d)).astype(dtype)
+    q[..., 9] = 200
+    got = run(ctx, plain, table, [0, new], lens, q).astype(np.float64)
+    want, size, _ = exact(plain, table, [0, new], lens, q, 0.125)
+    step = 2.0**-23.97 if dtype == "float32" else 2.0**-15.98 if new * group < 64 else 0.0
+    off = 6 * 200 * step / np.sqrt(3) * np.sqrt(64) * 1.75 * 0.125
+    assert (np.abs(got - want).max(2) <= (REL[dtype] + 2 * off) * size).all()
+
+
 def test_a_wider_table_takes_the_same_kernel(ctx):
     """A table with room for more tokens than the streams have: same pages, same bits."""
     rng = np.random.default_rng(14)
