@@ -8,8 +8,8 @@
 // append, block by block: s' = max(s, amax * (1/127)) with s = 0 where the block's
 // first slot is among the new tokens; the block's earlier quants become
 // rint(q * (s / s')) where s' > s, the new ones rint(x * (1 / s')). All in
-// IEEE fp32, so the stored bytes are defined to the bit. NaN counts as 0 and
-// infinities as the largest finite value of the block.
+// IEEE fp32, so the stored bytes are defined to the bit. NaN counts as 0, and a
+// block with an infinity has the scale FLT_MAX * (1/127): 127 stands for it.
 //
 // Bound: HBM, then the conversions. One warp holds one block of one head and
 // side: each lane owns d_head / 32 neighbouring channels of all 16 tokens, so a

@@ -11,8 +11,9 @@
 // Every operation is one IEEE fp32 rounding in this order, so the values do
 // not depend on which of the two entry points computes them.
 //
-// Bound: HBM, one pass over the logits (and, for process, one write). A CTA
-// works on windows of 256 threads x NV 16-byte vectors of one row: the logits
+// Bound: the arithmetic of the rules where they are all on, else HBM: one pass
+// over the logits (and, for process, one write). The history is read once for
+// each window, from L2. A CTA works on windows of 256 threads x NV 16-byte vectors of one row: the logits
 // of the window are loaded first, the history is counted into a table of the
 // window's tokens in shared memory while they arrive (integer adds: the order
 // does not matter), and every rule is applied in registers. Rows start at any
@@ -267,7 +268,7 @@ struct Window {
     }
 };
 
-// (Four blocks an SM: 14.8 us for 128 rows of 51866 in f32; five 17.9 and six 18.6, with spills.)
+// (Four blocks an SM: 14.8 to 16.4 us for 128 rows of 51866 in f32; five 17.9 and six 18.6, with spills.)
 template <typename T, int NV>
 __global__ void __launch_bounds__(LG_THREADS, 4) logits_process_kernel(const T* logits, int64_t ld, int vocab,
                                                                        Rules R, T* out, int64_t out_ld) {
@@ -746,8 +747,8 @@ void check_logits(const vkb_context* ctx, const void* logits, int dtype, int64_t
         fail(VKB_ERROR_INVALID_ARGUMENT, "logits: misaligned logits");
 }
 
-// 16-byte vectors of a thread. process, 128 rows of 51866 (f32): 2 vectors 17.2 us, 4 15.5 (14.8 with four blocks an
-// SM). Selection, 256 rows of 131071 (f16): 2 vectors 108 us, 3 107, 4 104 (fewer looks at a history of 2048 tokens).
+// 16-byte vectors of a thread. process, 128 rows of 51866 (f32): 2 vectors 17.2 us, 4 15.5 (14.8 to 16.4 with four blocks
+// an SM); the same in f16: 1 vector 23.4, 2 21.3, 4 26. Selection, 256 rows of 131071 (f16): 2 vectors 108 us, 3 107, 4 104 (fewer looks at a history of 2048 tokens).
 constexpr int NV_F32 = 4, NV_F16 = 2, NV_TOPK = 4;
 constexpr int64_t ROWS_PER_LAUNCH = 32768;  // grid.y
 

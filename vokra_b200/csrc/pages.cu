@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(PLAN) pages_plan_kernel(Pool P, const int32_t*
             W.copy[s] = copy;
         }
         taken += total;
-        if (taken > P.n_pages) break;  // more than there are (the sum stays far from 2^31)
+        if (taken > P.n_pages) break;  // more than there are (a stream takes ld at most, so no sum passes n_seq * ld < 2^31)
     }
     __syncthreads();
     if (why == 0 && taken > 0) {
