@@ -29,7 +29,7 @@
 // above fp32's smallest number in the sum.
 //
 // Measured: 4 prompts of up to 2047 tokens over up to 12000 keys, 8 x 4 heads of
-// 128: 687 us, 777 TFLOP/s, 47% of cuBLAS.
+// 128: 680 us, 785 TFLOP/s, 47% of cuBLAS.
 #include "bkv_attn.cuh"
 #include "tc_ptx.cuh"
 #include <algorithm>
@@ -388,9 +388,6 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             }
             ids_next = ids_of(j + 2);
         }
-        // The last steps' buffers are given back too: the block does not end before those arrivals.
-        for (int j = max(0, n_steps - 2); j < n_steps && ok; ++j)
-            if (2 * j + 1 < n_half && !ptx::mbar_wait(&empty[j & 1], (j >> 1) & 1)) ok = false;
     } else if (n_steps > 0) {
         // ---- the products, by the whole warp in step. Half i of a tile's keys has its scores in half i % 2 of the tile's
         // columns, so S of the next half is made while this one's softmax runs. Tile t is at S of half s_at[t] and P.V of
@@ -446,13 +443,13 @@ __global__ void __launch_bounds__(THREADS, 1) bkv_prompt_kernel(BkvAttn A, int* 
             }
         }
     }
-    if (!ok) {
-        atomicExch(err, 1);
-        // products under way end before the block does
-        if (warp == 15) {
-            ptx::mma_commit_warp(ended);
-            ptx::mbar_wait(ended, 0);
-        }
+    if (!ok) atomicExch(err, 1);
+    __syncwarp();
+    if (warp == 15) {
+        // The last commit of all: products and arrivals (the last steps' buffers are given back to nobody) that are under
+        // way, where a wait gave up too, end before the block does.
+        ptx::mma_commit_warp(ended);
+        ptx::mbar_wait(ended, 0);
     }
     __syncwarp();
     ptx::tc_fence_before();
